@@ -215,6 +215,68 @@ ENGINE_API EngineStatus pdefa_batch_submit_u8(PdefaBatchRunner* runner, const ui
  * ENGINE_ERR_RUNTIME (once) instead of leaving its arrays silently unwritten. */
 ENGINE_API EngineStatus pdefa_batch_wait(PdefaBatchRunner* runner, int64_t ticket);
 
+/* ---- Language-model operators (no counterpart in the reference) ----
+ * Device pointers on `device` (made current for the call, the caller's device is put
+ * back); strides in elements; types are EngineDType codes. Each call checks its
+ * arguments, enqueues on `stream` and returns: no synchronisation. Sizes of 0 are no
+ * error and write nothing. */
+
+/* h = x + residual in 32 bits (d_residual may be NULL);
+ * y = h * weight / sqrt(mean over the row of h^2 + eps).
+ * dtype (F32, F16, BF16) is the type of x, residual, h and y; weight is of that type
+ * or F32. d_h (may be NULL, may be d_x or d_residual itself) receives h rounded to
+ * dtype; y is computed from the unrounded h. With d_scales the output is 8-bit: d_y
+ * holds e4m3 bytes, d_scales one float for each 128 columns of a row,
+ * scale = max(largest |y| of the 128, 1e-10) / 448, byte = e4m3(y / scale). A row with
+ * a NaN or an infinity gives NaN. */
+ENGINE_API EngineStatus engine_rms_norm_device(const void* d_x, int64_t x_stride, const void* d_residual,
+                                               int64_t residual_stride, const void* d_weight, void* d_h,
+                                               int64_t h_stride, void* d_y, int64_t y_stride, float* d_scales,
+                                               int64_t scales_stride, int64_t rows, int64_t cols, int32_t dtype,
+                                               int32_t weight_dtype, float eps, int32_t device, void* stream);
+
+/* out[m, n] = sum over blocks kb of 128 k of
+ *             a_scales[m, kb] * b_scales[n / 128, kb] * (sum over the block of a[m, k] * b[n, k])
+ * a: [m, k] and b: [n, k] e4m3 bytes; out F32, F16 or BF16. A last block of k or n may
+ * be partial. Operands whose base or row stride is not a multiple of 16 bytes are
+ * copied into memory of the stream-ordered pool first. */
+ENGINE_API EngineStatus engine_matmul_fp8_device(const void* d_a, int64_t lda, const float* d_a_scales,
+                                                 int64_t lda_scales, const void* d_b, int64_t ldb,
+                                                 const float* d_b_scales, int64_t ldb_scales, void* d_out, int64_t ldo,
+                                                 int32_t out_dtype, int64_t m, int64_t n, int64_t k, int32_t device,
+                                                 void* stream);
+/* The same with one b (and b_scales) per expert, b_expert_stride and
+ * b_scales_expert_stride elements apart: rows d_offsets[e] .. d_offsets[e + 1] - 1 of a
+ * (offsets in device memory, rising, experts + 1 of them) meet expert e's. Rows of no
+ * expert give 0. The row counts are read on the GPU: the host never waits for them.
+ * Offsets are brought into 0 .. rows; where one is below its predecessor, its expert
+ * has no rows and the result for rows named twice is that of one of their experts. */
+ENGINE_API EngineStatus engine_matmul_grouped_fp8_device(const void* d_a, int64_t lda, const float* d_a_scales,
+                                                         int64_t lda_scales, const void* d_b, int64_t ldb,
+                                                         int64_t b_expert_stride, const float* d_b_scales,
+                                                         int64_t ldb_scales, int64_t b_scales_expert_stride,
+                                                         const int32_t* d_offsets, int64_t experts, void* d_out,
+                                                         int64_t ldo, int32_t out_dtype, int64_t rows, int64_t n,
+                                                         int64_t k, int32_t device, void* stream);
+
+/* One token per row of d_logits [rows, vocab] (F32, F16 or BF16; NaN counts as -inf).
+ * w = exp((logit - largest) / temperature), Z = sum of w. In the order of falling
+ * logits (equal ones by rising index) a token is kept if fewer than top_k tokens come
+ * before it, the mass before it is below top_p * Z, w >= min_p and w > 0; the first
+ * token is always kept. Of the kept tokens the one with the largest w / noise wins
+ * (lowest index among equals): with noise [rows, vocab] of independent exponential
+ * variates, token i is drawn with probability w_i / (sum of kept w). Negative or NaN
+ * noise takes its token out of the race.
+ * d_temperature, d_top_k, d_top_p, d_min_p: one value per row, or NULL (1, off, off,
+ * off). A temperature that is not above 0 picks the first token; top_k <= 0, top_p >= 1
+ * and min_p <= 0 are off. d_tokens[row]: the token, -1 where every logit is -inf;
+ * d_probs[row] (may be NULL): its w / Z (temperature 0: that of temperature 1), or 0. */
+ENGINE_API EngineStatus engine_sample_device(const void* d_logits, int64_t logits_stride, int32_t dtype,
+                                             const float* d_noise, int64_t noise_stride, const float* d_temperature,
+                                             const int32_t* d_top_k, const float* d_top_p, const float* d_min_p,
+                                             int64_t rows, int64_t vocab, int32_t* d_tokens, float* d_probs,
+                                             int32_t device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

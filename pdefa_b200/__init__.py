@@ -18,6 +18,7 @@ from .api import (  # noqa: F401
     zeros,
 )
 from .batch import BatchInference  # noqa: F401
+from .lm import ops_matmul_fp8, ops_matmul_grouped_fp8, ops_rms_norm, ops_rms_norm_fp8, ops_sample  # noqa: F401
 
 __all__ = [
     "PdefaError", "PreprocessMeta", "Box", "Tensor", "TensorInfo", "Context", "Model", "Session", "Image",
@@ -30,6 +31,7 @@ __all__ = [
     "ops_sigmoid", "ops_tanh", "ops_gelu", "ops_clip", "ops_softmax",
     "ops_reduce_max", "ops_reduce_sum", "ops_reduce_mean",
     "ops_argmax", "ops_gather", "ops_reshape", "ops_transpose", "ops_concat", "ops_stack",
+    "ops_rms_norm", "ops_rms_norm_fp8", "ops_matmul_fp8", "ops_matmul_grouped_fp8", "ops_sample",
     "random_randn", "random_rand", "randn", "rand", "zeros", "ones", "empty", "from_list",
     "load", "EngineModel", "BatchInference", "FP32", "TF32", "BF16",
 ]

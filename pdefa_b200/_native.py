@@ -93,6 +93,12 @@ _SIGS = {
     "engine_ops_mul": ([vp, vp, P(vp)], C.c_int), "engine_ops_div": ([vp, vp, P(vp)], C.c_int),
     "engine_ops_matmul": ([vp, vp, vp], C.c_int), "engine_ops_matmul_ex": ([vp, vp, vp, i32], C.c_int),
     "engine_gemm_f32_device": ([vp, vp, vp, i64, i64, i64, i32, vp], C.c_int),
+    "engine_rms_norm_device": ([vp, i64, vp, i64, vp, vp, i64, vp, i64, vp, i64, i64, i64, i32, i32, f32, i32, vp],
+                               C.c_int),
+    "engine_matmul_fp8_device": ([vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, i32, i64, i64, i64, i32, vp], C.c_int),
+    "engine_matmul_grouped_fp8_device": ([vp, i64, vp, i64, vp, i64, i64, vp, i64, i64, vp, i64, vp, i64, i32, i64,
+                                          i64, i64, i32, vp], C.c_int),
+    "engine_sample_device": ([vp, i64, i32, vp, i64, vp, vp, vp, vp, i64, i64, vp, vp, i32, vp], C.c_int),
     "engine_ops_relu": ([vp], C.c_int), "engine_ops_silu": ([vp], C.c_int),
     "engine_ops_sigmoid": ([vp], C.c_int), "engine_ops_tanh": ([vp], C.c_int),
     "engine_ops_gelu": ([vp], C.c_int), "engine_ops_clip": ([vp, f32, f32], C.c_int),

@@ -198,4 +198,57 @@ size_t gemm_device_scratch_bytes(int64_t m, int64_t n, int64_t k, int precision)
 void gemm_device(const float* d_a, const float* d_b, float* d_c, int64_t m, int64_t n, int64_t k, int precision,
                  void* scratch, cudaStream_t s);
 
+// ---------------------------------------------------------------------------
+// Language-model operators. Type codes are EngineDType values (F32, F16, BF16).
+// ---------------------------------------------------------------------------
+// Rows of x (+ residual) normalised by their root mean square and scaled by weight
+// [cols]; strides in elements. h_out (may be null) receives x + residual, and may be
+// x or residual itself. quantize: y holds e4m3 bytes and scales one float per 128 columns.
+struct RmsNormArgs {
+    const void* x = nullptr;
+    const void* residual = nullptr;
+    const void* weight = nullptr;
+    void* h_out = nullptr;
+    void* y = nullptr;
+    float* scales = nullptr;
+    int64_t rows = 0, cols = 0;
+    int64_t x_stride = 0, residual_stride = 0, h_stride = 0, y_stride = 0, scales_stride = 0;
+    float eps = 0.0f;
+    int dtype = 0, weight_dtype = 0;   // weight: x's type or F32
+    int quantize = 0;
+};
+void launch_rms_norm(const RmsNormArgs& a, cudaStream_t s);
+
+// out[m, n] = sum_kb a_scales[m, kb] * b_scales[n / 128, kb] * sum_{k in kb} a[m, k] b[n, k]
+// over e4m3 bytes. offsets (device, may be null): expert e's rows of a are
+// offsets[e] .. offsets[e + 1] - 1 and meet b + e * b_expert; rows of no expert give 0.
+struct MatmulFp8Args {
+    const void* a = nullptr;
+    const void* b = nullptr;
+    const float* a_scales = nullptr;
+    const float* b_scales = nullptr;
+    const int32_t* offsets = nullptr;
+    void* out = nullptr;
+    int64_t m = 0, n = 0, k = 0, experts = 1;
+    int64_t lda = 0, ldb = 0, lda_scales = 0, ldb_scales = 0, ldo = 0;
+    int64_t b_expert = 0, b_scales_expert = 0;
+    int out_dtype = 0;
+};
+void launch_matmul_fp8(const MatmulFp8Args& p, cudaStream_t s);
+
+// One token per row of logits [rows, vocab]; see engine_sample_device.
+struct SampleArgs {
+    const void* logits = nullptr;
+    const float* noise = nullptr;
+    const float* temperature = nullptr;
+    const int32_t* top_k = nullptr;
+    const float* top_p = nullptr;
+    const float* min_p = nullptr;
+    int32_t* tokens = nullptr;
+    float* probs = nullptr;
+    int64_t rows = 0, vocab = 0, logits_stride = 0, noise_stride = 0;
+    int dtype = 0;
+};
+void launch_sample(const SampleArgs& a, cudaStream_t s);
+
 }  // namespace pb
