@@ -249,8 +249,8 @@ ENGINE_API EngineStatus engine_matmul_fp8_device(const void* d_a, int64_t lda, c
  * b_scales_expert_stride elements apart: rows d_offsets[e] .. d_offsets[e + 1] - 1 of a
  * (offsets in device memory, rising, experts + 1 of them) meet expert e's. Rows of no
  * expert give 0. The row counts are read on the GPU: the host never waits for them.
- * Offsets are brought into 0 .. rows; where one is below its predecessor, its expert
- * has no rows and the result for rows named twice is that of one of their experts. */
+ * An offset outside 0 .. rows or below one before it counts as the nearest value that
+ * is not. 1024 experts at most. */
 ENGINE_API EngineStatus engine_matmul_grouped_fp8_device(const void* d_a, int64_t lda, const float* d_a_scales,
                                                          int64_t lda_scales, const void* d_b, int64_t ldb,
                                                          int64_t b_expert_stride, const float* d_b_scales,

@@ -73,7 +73,7 @@ EngineStatus matmul_fp8(MatmulFp8Args p, int32_t device, void* stream) {
     need_stride(p.ldo, p.n, p.m, "matmul_fp8: stride of the output");
     need_aligned(p.out, align_of(p.out_dtype), "matmul_fp8: the output is not aligned");
     if (p.offsets) {
-        need(p.experts >= 1 && p.experts <= 65535, ENGINE_ERR_INVALID_SHAPE, "matmul_fp8: 1 to 65535 experts");
+        need(p.experts >= 1 && p.experts <= 1024, ENGINE_ERR_INVALID_SHAPE, "matmul_fp8: 1 to 1024 experts");
         need_aligned(p.offsets, 4, "matmul_fp8: the offsets are not aligned");
         need_input_stride(p.b_expert, p.experts, "matmul_fp8: expert stride of b");
         need_input_stride(p.b_scales_expert, p.experts, "matmul_fp8: expert stride of b's scales");

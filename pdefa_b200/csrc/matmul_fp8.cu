@@ -4,25 +4,169 @@
 //               (sum over the 128 k of block kb of a[m, k] * b[n, k])
 //
 // a is [M, K] (rows are tokens), b is [N, K] (a weight as it is stored), or
-// [experts, N, K] with `offsets` giving each expert's range of rows of a. The inner
-// sum of a block is exact products in 32-bit accumulation; blocks are joined in
-// 32 bits.
+// [experts, N, K] with `offsets` giving each expert's range of rows of a.
+//
+// One warp-specialised tcgen05 kernel for all of it. A tile is 128 rows of the weight
+// (the M side of the instruction, its 128 TMEM lanes) times BT tokens (its N side, BT
+// TMEM columns), so a handful of tokens costs a narrow tile and not 128 padded rows.
+// Scales change with every 128 k, so an accumulator cannot run through K on the tensor
+// core: each k-block (one 128-byte swizzled row per operand row, four instructions of
+// K = 32) goes into a fresh TMEM buffer, and the epilogue warps add buffer * scale to
+// 32-bit sums in registers, while the tensor core fills the next buffer. The tile's
+// weight rows share one scale per k-block (tiles start at multiples of 128), the
+// tokens have one each; their products come from shared memory as one broadcast load
+// per four columns, and the sum is one packed fp32x2 multiply-add per two columns.
+#include <algorithm>
+#include <cuda.h>
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 
 #include "common.h"
 #include "device_common.cuh"
+#include "tc_common.cuh"
 
 namespace pb {
 
 namespace {
 
-constexpr int kBlock = 128;
+constexpr int kBlock = 128;             // k per scale, and bytes of an operand row per stage
+constexpr int kTileN = 128;             // weight rows of a tile
+constexpr int kScaleChunk = 8;          // k-blocks of scales staged at a time (one 32-byte sector per token)
+constexpr uint32_t kABytes = kTileN * kBlock;
+constexpr uint32_t kBarrierBytes = 512;
 
-__device__ __forceinline__ float e4m3(uint8_t v) {
-    __nv_fp8_e4m3 f;
-    f.__x = v;
-    return (float)f;
+struct TcArgs {
+    const int32_t* offsets;             // null: one weight
+    int experts, m, n, nkb;             // nkb: k-blocks
+    int n_tiles, m_tiles;               // m_tiles: token tiles (one weight)
+    int stages, split;
+    const float* sa; int64_t lda_scales;
+    const float* sb; int64_t ldb_scales, sb_expert;
+    void* out; int64_t ldo; int out_dtype;
+    uint32_t table_bytes;               // the experts' tile table in shared memory (12 KB for the most experts)
+    int* err;
+    long long wait_limit;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
+    float v;
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}"
+                 : "=f"(v) : "r"(addr), "r"(rank) : "memory");
+    return v;
+}
+
+// A bounded wait of a whole warp, with one answer for all lanes.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, long long limit) {
+    return __all_sync(~0u, mbar_wait_bounded(bar, parity, limit));
+}
+
+// One k-block: four K = 32 products into a fresh accumulator, then a commit to the
+// ring slot's and to the accumulator's barrier.
+__device__ __forceinline__ void mma_kblock(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint64_t* slot_free,
+                                           uint64_t* acc_full) {
+    asm volatile(
+        "{\n\t.reg .pred pf, pt;\n\t.reg .b64 a1, b1, a2, b2, a3, b3;\n\t"
+        "setp.ne.u32 pf, 0, 0;\n\tsetp.eq.u32 pt, 0, 0;\n\t"
+        "add.s64 a1, %1, 2;\n\tadd.s64 b1, %2, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 b2, %2, 4;\n\t"
+        "add.s64 a3, %1, 6;\n\tadd.s64 b3, %2, 6;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, pf;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a1, b1, %3, pt;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a2, b2, %3, pt;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a3, b3, %3, pt;\n\t"
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%4];\n\t"
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t}"
+        ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(smem_u32(slot_free)), "r"(smem_u32(acc_full))
+        : "memory");
+}
+
+template <int BT>
+struct Shape {
+    static constexpr int kEpi = BT >= 128 ? 8 : 4;                  // epilogue warps
+    static constexpr int kThreads = 128 + 32 * kEpi;
+    static constexpr int kCols = BT * 4 / kEpi;                     // columns of an epilogue thread
+    static constexpr int kBufs = BT == 256 ? 2 : 4;                 // TMEM accumulators
+    static constexpr int kTmemCols = kBufs * BT;                    // 64 .. 512
+    static constexpr uint32_t kBBytes = BT * kBlock;
+    static constexpr uint32_t kScaleBytes = kScaleChunk * BT * 4;   // of one of two chunks
+};
+
+struct Tile {
+    int expert, row0, rows, n0;         // first token, tokens that belong to the tile, first weight row
+};
+
+// The experts' rows: [first row | end | token tiles before it] for each, in shared memory;
+// returns the number of token tiles. An offset outside 0 .. m or below one before it
+// counts as the nearest value that is not, so every row has one expert at most. One warp.
+template <int BT>
+__device__ __forceinline__ int build_table(const TcArgs& p, int* table) {
+    const int lane = threadIdx.x & 31;
+    int before = 0, least = 0;
+    for (int e0 = 0; e0 < p.experts; e0 += 32) {
+        const int e = e0 + lane;
+        int lo = 0, hi = 0;
+        if (e < p.experts) {
+            lo = min(max(p.offsets[e], 0), p.m);
+            hi = min(max(p.offsets[e + 1], 0), p.m);
+        }
+        lo = max(lo, least);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) lo = max(lo, __shfl_up_sync(~0u, lo, o));
+        hi = max(hi, lo);
+        least = __shfl_sync(~0u, hi, 31);
+        const int rows = hi - lo, tiles = e < p.experts ? rows / BT + (rows % BT != 0) : 0;
+        int sum = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(~0u, sum, o);
+            if (lane >= o) sum += v;
+        }
+        if (e < p.experts) {
+            table[e] = lo;
+            table[p.experts + e] = hi;
+            table[2 * p.experts + e] = before + sum - tiles;
+        }
+        before += __shfl_sync(~0u, sum, 31);
+    }
+    return before;
+}
+
+// Tiles are numbered with the token tiles of an expert innermost, so that CTAs that run
+// together read the same weight rows.
+template <int BT>
+__device__ __forceinline__ Tile tile_of(const TcArgs& p, const int* table, int token_tiles, int64_t t) {
+    Tile r;
+    if (!p.offsets) {
+        const int nt = (int)(t / p.m_tiles);
+        r.expert = 0;
+        r.row0 = (int)(t - (int64_t)nt * p.m_tiles) * BT;
+        r.rows = min(BT, p.m - r.row0);
+        r.n0 = nt * kTileN;
+        return r;
+    }
+    const int* before = table + 2 * p.experts;
+    const int u = (int)(t / p.n_tiles);             // lies in the expert's range of token tiles
+    int lo = 0, hi = p.experts - 1;                 // last expert with before <= u
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (before[mid] <= u) lo = mid;
+        else hi = mid - 1;
+    }
+    const int mine = (lo + 1 < p.experts ? before[lo + 1] : token_tiles) - before[lo];
+    const int64_t local = t - (int64_t)before[lo] * p.n_tiles;
+    const int nt = (int)(local / mine);
+    r.expert = lo;
+    r.row0 = table[lo] + (int)(local - (int64_t)nt * mine) * BT;
+    r.rows = min(BT, table[p.experts + lo] - r.row0);
+    r.n0 = nt * kTileN;
+    return r;
 }
 
 __device__ __forceinline__ void store_out(void* out, int dtype, int64_t i, float v) {
@@ -31,46 +175,396 @@ __device__ __forceinline__ void store_out(void* out, int dtype, int64_t i, float
     else static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
 }
 
-// One thread per output.
-__global__ void __launch_bounds__(256)
-matmul_fp8_simple_kernel(MatmulFp8Args p) {
-    const int64_t n = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
-    const int64_t m = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5);
-    if (m >= p.m || n >= p.n) return;
-    const uint8_t* b = static_cast<const uint8_t*>(p.b);
-    const float* sb = p.b_scales;
-    if (p.offsets) {
-        int e = 0;
-        while (e < p.experts && !(p.offsets[e] <= m && m < p.offsets[e + 1])) ++e;
-        if (e == p.experts) {
-            store_out(p.out, p.out_dtype, m * p.ldo + n, 0.0f);
-            return;
+// Roles: warp 0 brings operands (TMA), warp 1 issues the products and owns TMEM, warp 2
+// brings scales, warps 4 and up are the epilogue. Every wait is bounded; one that runs
+// out records a code in the device's error word and ends its role, after which the
+// others' waits run out too; loads and products in flight are waited for before exit.
+// SPLIT: the CTAs of a cluster take the k-blocks of one tile in equal parts and join
+// their sums through distributed shared memory in rank order.
+template <int BT, bool SPLIT>
+__global__ void __launch_bounds__(Shape<BT>::kThreads, 1)
+matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmA, const TcArgs p) {
+    using S = Shape<BT>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    uint8_t* const smem = smem_raw + (base - raw);
+    const int stages = p.stages;
+    // [weight slots | token slots | scales | barriers | table], slots 1024-aligned
+    const uint32_t ring_b = base + (uint32_t)stages * kABytes;
+    float* const scales = reinterpret_cast<float*>(smem + (size_t)stages * (kABytes + S::kBBytes));
+    uint64_t* const full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(scales) + 2 * S::kScaleBytes);
+    uint64_t* const empty = full + stages;
+    uint64_t* const tfull = empty + stages;
+    uint64_t* const tempty = tfull + S::kBufs;
+    uint64_t* const sfull = tempty + S::kBufs;
+    uint64_t* const sempty = sfull + 2;
+    uint64_t* const mma_done = sempty + 2;
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
+    int* const tile_count = reinterpret_cast<int*>(tmem_slot + 1);
+    int* const table = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(full) + kBarrierBytes);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < stages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < S::kBufs; ++i) { mbar_init(&tfull[i], 1); mbar_init(&tempty[i], S::kEpi); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&sfull[i], 1); mbar_init(&sempty[i], S::kEpi); }
+        mbar_init(mma_done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)S::kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (warp == 2) {
+        const int n = p.offsets ? build_table<BT>(p, table) : p.m_tiles;
+        if (lane == 0) *tile_count = n;
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+    const int token_tiles = *tile_count;
+    const int64_t total = (int64_t)token_tiles * p.n_tiles;
+
+    // this CTA's tiles and, of each, its k-blocks
+    const uint32_t rank = SPLIT ? cluster_rank() : 0;
+    const int64_t t0 = SPLIT ? blockIdx.x / p.split : blockIdx.x;
+    const int64_t tstep = SPLIT ? total : gridDim.x;        // SPLIT: one tile per cluster
+    const int kb0 = SPLIT ? (int)((int64_t)p.nkb * rank / p.split) : 0;
+    const int kb1 = SPLIT ? (int)((int64_t)p.nkb * (rank + 1) / p.split) : p.nkb;
+
+    float acc[S::kCols];
+    Tile mine{0, 0, 0, 0};
+    bool failed = false;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            RingPos rp;
+            int64_t it = 0;
+            for (int64_t t = t0; t < total && !failed; t += tstep) {
+                const Tile tl = tile_of<BT>(p, table, token_tiles, t);
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    const int st = rp.slot;
+                    if (rp.wrapped && !mbar_wait_bounded(&empty[st], rp.phase ^ 1u, p.wait_limit)) {
+                        atomicExch(p.err, 21);
+                        failed = true;
+                        break;
+                    }
+                    rp.next(stages);
+                    ++it;
+                    mbar_expect_tx(&full[st], kABytes + S::kBBytes);
+                    tma_load_3d(base + (uint32_t)st * kABytes, &tmB, &full[st], kb * kBlock, tl.n0, tl.expert);
+                    tma_load_2d(ring_b + (uint32_t)st * S::kBBytes, &tmA, &full[st], kb * kBlock, tl.row0);
+                }
+            }
+            // the last load of every slot has landed before the CTA may exit
+            for (int64_t k = it > stages ? it - stages : 0; k < it; ++k)
+                if (!mbar_wait_bounded(&full[k % stages], (uint32_t)((k / stages) & 1))) atomicExch(p.err, 22);
         }
-        b += e * p.b_expert;
-        sb += e * p.b_scales_expert;
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            // f32 accumulator, e4m3 operands, N = BT, M = 128
+            const uint32_t idesc = (1u << 4) | ((uint32_t)(BT >> 3) << 17) | ((uint32_t)(kTileN >> 4) << 24);
+            RingPos rp, ap;
+            for (int64_t t = t0; t < total && !failed; t += tstep) {
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    const int st = rp.slot, buf = ap.slot;
+                    if ((ap.wrapped && !mbar_wait_bounded(&tempty[buf], ap.phase ^ 1u, p.wait_limit)) ||
+                        !mbar_wait_bounded(&full[st], rp.phase, p.wait_limit)) {
+                        atomicExch(p.err, 23);
+                        failed = true;
+                        break;
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    mma_kblock(tmem + (uint32_t)(buf * BT), make_smem_desc(base + (uint32_t)st * kABytes, 128),
+                               make_smem_desc(ring_b + (uint32_t)st * S::kBBytes, 128), idesc, &empty[st], &tfull[buf]);
+                    rp.next(stages);
+                    ap.next(S::kBufs);
+                }
+            }
+            umma_commit(mma_done);
+        }
+        __syncwarp();
+    } else if (warp == 2) {
+        // scales: chunk c holds sa[token, kb] * sb[kb] for kScaleChunk k-blocks, [kb][token]
+        RingPos cp;
+        for (int64_t t = t0; t < total && !failed; t += tstep) {
+            const Tile tl = tile_of<BT>(p, table, token_tiles, t);
+            const float* sa = p.sa + (int64_t)tl.row0 * p.lda_scales;
+            const float* sb = p.sb + tl.expert * p.sb_expert + (tl.n0 / kTileN) * p.ldb_scales;
+            for (int kc = kb0; kc < kb1 && !failed; kc += kScaleChunk) {
+                float w[kScaleChunk];
+#pragma unroll
+                for (int j = 0; j < kScaleChunk; ++j) w[j] = kc + j < kb1 ? __ldg(sb + kc + j) : 0.0f;
+                if (cp.wrapped && !warp_wait(&sempty[cp.slot], cp.phase ^ 1u, p.wait_limit)) {
+                    if (lane == 0) atomicExch(p.err, 24);
+                    failed = true;
+                    break;
+                }
+                float* dst = scales + cp.slot * (kScaleChunk * BT);
+#pragma unroll(BT >= 128 ? 4 : 1)
+                for (int i = lane; i < BT; i += 32) {
+                    float v[kScaleChunk];
+#pragma unroll
+                    for (int j = 0; j < kScaleChunk; ++j)
+                        v[j] = i < tl.rows && kc + j < kb1 ? __ldg(sa + i * p.lda_scales + kc + j) : 0.0f;
+#pragma unroll
+                    for (int j = 0; j < kScaleChunk; ++j) dst[j * BT + i] = v[j] * w[j];
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sfull[cp.slot]);
+                cp.next(2);
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        const int q = warp & 3;                           // TMEM lane quarter
+        const int c0 = ((warp - 4) >> 2) * S::kCols;      // first column of this warp's group
+        const uint32_t lanes = (uint32_t)(q * 32) << 16;
+        RingPos ap, cp;
+        for (int64_t t = t0; t < total && !failed; t += tstep) {
+            mine = tile_of<BT>(p, table, token_tiles, t);
+#pragma unroll
+            for (int i = 0; i < S::kCols; ++i) acc[i] = 0.0f;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                const int in_chunk = (kb - kb0) % kScaleChunk;
+                if ((in_chunk == 0 && !warp_wait(&sfull[cp.slot], cp.phase, p.wait_limit)) ||
+                    !warp_wait(&tfull[ap.slot], ap.phase, p.wait_limit)) {
+                    if (lane == 0) atomicExch(p.err, 25);
+                    failed = true;
+                    break;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t src = tmem + lanes + (uint32_t)(ap.slot * BT + c0);
+                const float4* sc = reinterpret_cast<const float4*>(scales + cp.slot * (kScaleChunk * BT) + in_chunk * BT + c0);
+                uint32_t r[2][16];
+                tmem_ld16_async(src, r[0]);
+#pragma unroll
+                for (int c = 0; c < S::kCols / 16; ++c) {
+                    tmem_wait_ld();
+                    if (c + 1 < S::kCols / 16) tmem_ld16_async(src + (c + 1) * 16, r[(c + 1) & 1]);
+                    else {
+                        // everything is in registers: the tensor core may refill the buffer
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&tempty[ap.slot]);
+                    }
+                    const uint32_t(&v)[16] = r[c & 1];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float4 s4 = sc[c * 4 + j];
+                        float* d = acc + c * 16 + j * 4;
+                        const float2 lo = __ffma2_rn(make_float2(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1])),
+                                                     make_float2(s4.x, s4.y), make_float2(d[0], d[1]));
+                        const float2 hi = __ffma2_rn(make_float2(__uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3])),
+                                                     make_float2(s4.z, s4.w), make_float2(d[2], d[3]));
+                        d[0] = lo.x; d[1] = lo.y; d[2] = hi.x; d[3] = hi.y;
+                    }
+                }
+                ap.next(S::kBufs);
+                if (in_chunk == kScaleChunk - 1 || kb == kb1 - 1) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sempty[cp.slot]);
+                    cp.next(2);
+                }
+            }
+            if (SPLIT || failed) continue;
+            const int n = mine.n0 + q * 32 + lane;
+            if (n < p.n) {
+#pragma unroll
+                for (int i = 0; i < S::kCols; ++i)
+                    if (c0 + i < mine.rows) store_out(p.out, p.out_dtype, (int64_t)(mine.row0 + c0 + i) * p.ldo + n, acc[i]);
+            }
+        }
+        if (!SPLIT && p.offsets) {
+            // rows before the first and after the last expert's
+            const int lo = table[0], hi = table[2 * p.experts - 1];
+            const int tid = threadIdx.x - 128;
+            for (int64_t i = (int64_t)blockIdx.x; i < (int64_t)lo + (p.m - hi); i += gridDim.x) {
+                const int64_t row = i < lo ? i : hi + (i - lo);
+                for (int n = tid; n < p.n; n += 32 * S::kEpi) store_out(p.out, p.out_dtype, row * p.ldo + n, 0.0f);
+            }
+        }
     }
-    const uint8_t* ar = static_cast<const uint8_t*>(p.a) + m * p.lda;
-    const uint8_t* br = b + n * p.ldb;
-    float sum = 0.0f;
-    for (int64_t k0 = 0; k0 < p.k; k0 += kBlock) {
-        float part = 0.0f;
-        const int64_t k1 = k0 + kBlock < p.k ? k0 + kBlock : p.k;
-        for (int64_t k = k0; k < k1; ++k) part = fmaf(e4m3(ar[k]), e4m3(br[k]), part);
-        sum = fmaf(part, p.a_scales[m * p.lda_scales + k0 / kBlock] * sb[n / kBlock * p.ldb_scales + k0 / kBlock], sum);
+
+    if (SPLIT) {
+        // Sums as [token][weight row] in the ring's memory: every load and product of
+        // this CTA is behind the epilogue's last accumulator.
+        float* const part = reinterpret_cast<float*>(smem);
+        const int q = warp & 3, c0 = ((warp - 4) >> 2) * S::kCols;
+        if (warp >= 4 && !failed) {
+#pragma unroll
+            for (int i = 0; i < S::kCols; ++i) part[(c0 + i) * kTileN + q * 32 + lane] = acc[i];
+        }
+        __syncwarp();
+        cluster_sync();
+        if (warp >= 4 && !failed) {
+            const int tid = threadIdx.x - 128;
+            const int per = BT / p.split, n = mine.n0 + (tid & 127);
+            for (int j = (int)rank * per + (tid >> 7); j < ((int)rank + 1) * per; j += S::kEpi / 4) {
+                if (j >= mine.rows || n >= p.n) continue;
+                float sum = 0.0f;
+                for (int c = 0; c < p.split; ++c) sum += ld_cluster(smem_u32(part + j * kTileN + (tid & 127)), c);
+                store_out(p.out, p.out_dtype, (int64_t)(mine.row0 + j) * p.ldo + n, sum);
+            }
+        }
+        __syncwarp();
+        cluster_sync();
     }
-    store_out(p.out, p.out_dtype, m * p.ldo + n, sum);
+
+    // TMEM is freed once every issued product has completed.
+    __syncthreads();
+    if (warp == 1) {
+        if (!mbar_wait_bounded(mma_done, 0) && lane == 0) atomicExch(p.err, 26);
+        __syncwarp();
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)S::kTmemCols) : "memory");
+    }
+}
+
+// Rows of bytes into rows of `ld` bytes (a multiple of 16), for operands that TMA cannot read.
+__global__ void __launch_bounds__(256)
+repack_rows_kernel(const uint8_t* src, int64_t ld_src, int64_t group_src, uint8_t* dst, int64_t ld, int64_t rows, int64_t cols,
+                   int64_t groups) {
+    for (int64_t r = blockIdx.x; r < rows * groups; r += gridDim.x) {
+        const uint8_t* s = src + (r / rows) * group_src + (r % rows) * ld_src;
+        for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) dst[r * ld + c] = s[c];
+    }
+}
+
+// Memory of the stream-ordered pool for the length of a call's work.
+struct PoolBuffer {
+    void* p = nullptr;
+    cudaStream_t s;
+    explicit PoolBuffer(cudaStream_t st) : s(st) {}
+    void* get(size_t n) { PB_CUDA(cudaMallocAsync(&p, n, s)); return p; }
+    ~PoolBuffer() { if (p) cudaFreeAsync(p, s); }
+};
+
+template <int BT, bool SPLIT>
+void launch_tc(const TcArgs& args, int64_t grid, const CUtensorMap& tmB, const CUtensorMap& tmA, int device, cudaStream_t s) {
+    using S = Shape<BT>;
+    TcArgs p = args;
+    const uint32_t fixed = 1024 + 2 * S::kScaleBytes + kBarrierBytes + p.table_bytes;
+    p.stages = (int)std::min<uint32_t>(12, (227u * 1024u - fixed) / (kABytes + S::kBBytes));
+    const size_t smem = fixed + (size_t)p.stages * (kABytes + S::kBBytes);
+    static bool ready[64] = {};
+    if (device >= 64 || !ready[device]) {
+        PB_CUDA(cudaFuncSetAttribute(matmul_fp8_kernel<BT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+        if (device < 64) ready[device] = true;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(S::kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)p.split;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = SPLIT ? 1 : 0;
+    PB_CUDA(cudaLaunchKernelEx(&cfg, matmul_fp8_kernel<BT, SPLIT>, tmB, tmA, p));
 }
 
 }  // namespace
 
-void launch_matmul_fp8(const MatmulFp8Args& p, cudaStream_t s) {
-    if (p.m == 0 || p.n == 0) return;
-    for (int64_t m0 = 0; m0 < p.m; m0 += 65535 * 8) {      // grid rows are limited to 65535
-        if (m0) fail(ENGINE_ERR_NOT_IMPL, "matmul_fp8: more than 524280 rows");
+void launch_matmul_fp8(const MatmulFp8Args& g, cudaStream_t s) {
+    if (g.m == 0 || g.n == 0) return;
+    if (g.k == 0) {
+        const size_t e = g.out_dtype == ENGINE_F32 ? 4 : 2;
+        PB_CUDA(cudaMemset2DAsync(g.out, (size_t)(g.m > 1 ? g.ldo : g.n) * e, 0, (size_t)g.n * e, (size_t)g.m, s));
+        return;
     }
-    dim3 grid((unsigned)((p.n + 31) / 32), (unsigned)((p.m + 7) / 8));
-    matmul_fp8_simple_kernel<<<grid, 256, 0, s>>>(p);
-    PB_CUDA(cudaGetLastError());
+    int device = 0;
+    PB_CUDA(cudaGetDevice(&device));
+    static int sm_count[64] = {};
+    int sms = device < 64 ? sm_count[device] : 0;
+    if (!sms) {
+        PB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+        if (device < 64) sm_count[device] = sms;
+    }
+
+    // TMA reads rows that start at multiples of 16 bytes and do not overlap; others are
+    // copied into such rows first.
+    const int64_t experts = g.offsets ? g.experts : 1;
+    const int64_t k16 = (g.k + 15) & ~int64_t(15);
+    auto plain = [&](const void* p, int64_t ld, int64_t rows) {
+        return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows <= 1 || (ld % 16 == 0 && ld >= g.k));
+    };
+    PoolBuffer mem_a(s), mem_b(s);
+    const void* a = g.a;
+    const void* b = g.b;
+    int64_t lda = g.m > 1 ? g.lda : k16, ldb = g.n > 1 ? g.ldb : k16, b_expert = experts > 1 ? g.b_expert : ldb * g.n;
+    if (!plain(g.a, g.lda, g.m)) {
+        a = mem_a.get((size_t)(g.m * k16));
+        repack_rows_kernel<<<(unsigned)std::min<int64_t>(g.m, 16 * sms), 256, 0, s>>>(
+            static_cast<const uint8_t*>(g.a), g.lda, 0, static_cast<uint8_t*>(mem_a.p), k16, g.m, g.k, 1);
+        PB_CUDA(cudaGetLastError());
+        lda = k16;
+    }
+    if (!plain(g.b, g.ldb, g.n) || (experts > 1 && (g.b_expert % 16 || g.b_expert < (g.n - 1) * ldb + g.k))) {
+        b = mem_b.get((size_t)(experts * g.n * k16));
+        repack_rows_kernel<<<(unsigned)std::min<int64_t>(experts * g.n, 16 * sms), 256, 0, s>>>(
+            static_cast<const uint8_t*>(g.b), g.ldb, g.b_expert, static_cast<uint8_t*>(mem_b.p), k16, g.n, g.k, experts);
+        PB_CUDA(cudaGetLastError());
+        ldb = k16;
+        b_expert = g.n * k16;
+    }
+
+    TcArgs p{};
+    p.offsets = g.offsets;
+    p.experts = (int)experts;
+    p.m = (int)g.m;
+    p.n = (int)g.n;
+    p.nkb = (int)((g.k + kBlock - 1) / kBlock);
+    p.n_tiles = (int)((g.n + kTileN - 1) / kTileN);
+    p.sa = g.a_scales; p.lda_scales = g.lda_scales;
+    p.sb = g.b_scales; p.ldb_scales = g.ldb_scales; p.sb_expert = g.offsets ? g.b_scales_expert : 0;
+    p.out = g.out; p.ldo = g.ldo; p.out_dtype = g.out_dtype;
+    p.table_bytes = g.offsets ? (uint32_t)(12 * experts + 15) & ~15u : 0;
+    p.err = device_error_word(device);
+    p.wait_limit = 1000000000LL;
+    p.split = 1;
+
+    // Tokens of a tile: the smallest width that holds the rows (an expert's average), so that
+    // few tokens do not pay for a wide tile's empty columns.
+    const int64_t rows = g.offsets ? (g.m + experts - 1) / experts : g.m;
+    const int bt = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+    p.m_tiles = (int)((g.m + bt - 1) / bt);
+
+    CUtensorMap tmA, tmB;
+    {
+        const uint64_t dims[2] = {(uint64_t)g.k, (uint64_t)g.m}, st[1] = {(uint64_t)lda};
+        const uint32_t box[2] = {kBlock, (uint32_t)bt};
+        if (!encode_box_map(&tmA, 1, 2, a, dims, st, box, true)) fail(ENGINE_ERR_INVALID_ARG, "matmul_fp8: tensor map of a refused");
+    }
+    {
+        const uint64_t dims[3] = {(uint64_t)g.k, (uint64_t)g.n, (uint64_t)experts}, st[2] = {(uint64_t)ldb, (uint64_t)b_expert};
+        const uint32_t box[3] = {kBlock, kTileN, 1};
+        if (!encode_box_map(&tmB, 1, 3, b, dims, st, box, true)) fail(ENGINE_ERR_INVALID_ARG, "matmul_fp8: tensor map of b refused");
+    }
+
+    // Token tiles there can be at most: one per expert with rows, and one per full tile.
+    const int64_t tiles = (g.offsets ? std::min<int64_t>(g.m, experts + g.m / bt) : p.m_tiles) * p.n_tiles;
+    // Few tiles: a cluster of 2, 4 or 8 CTAs per tile, as long as each still gets two k-blocks
+    // and the clusters fit the SMs at once.
+    int split = 1;
+    if (!g.offsets && bt <= 128)
+        while (split < 8 && tiles * split * 2 <= sms && p.nkb >= split * 4) split *= 2;
+    p.split = split;
+    const int64_t grid = split > 1 ? tiles * split : std::min<int64_t>(tiles, sms);
+    switch (bt) {
+        case 16: split > 1 ? launch_tc<16, true>(p, grid, tmB, tmA, device, s) : launch_tc<16, false>(p, grid, tmB, tmA, device, s); break;
+        case 32: split > 1 ? launch_tc<32, true>(p, grid, tmB, tmA, device, s) : launch_tc<32, false>(p, grid, tmB, tmA, device, s); break;
+        case 64: split > 1 ? launch_tc<64, true>(p, grid, tmB, tmA, device, s) : launch_tc<64, false>(p, grid, tmB, tmA, device, s); break;
+        case 128: split > 1 ? launch_tc<128, true>(p, grid, tmB, tmA, device, s) : launch_tc<128, false>(p, grid, tmB, tmA, device, s); break;
+        default: launch_tc<256, false>(p, grid, tmB, tmA, device, s); break;
+    }
 }
 
 }  // namespace pb

@@ -1,0 +1,65 @@
+// Device helpers of the tcgen05 kernels: ring positions, shared-memory descriptors, TMA
+// loads (none uses cluster multicast) and TMEM reads.
+#pragma once
+
+#include "device_common.cuh"
+
+namespace pb {
+
+// Position in a ring of n slots: slot index and the parity of the pass, advanced
+// without division. The pipeline roles are single threads (or one warp) that step
+// their rings once per k-block; a 64-bit division by a runtime ring size is a long
+// software sequence on the GPU and cost those threads thousands of cycles per tile.
+struct RingPos {
+    int slot = 0;
+    uint32_t phase = 0;     // completed passes & 1
+    bool wrapped = false;   // at least one full pass: every slot was used before
+    __device__ __forceinline__ void next(int n) {
+        if (++slot == n) { slot = 0; phase ^= 1u; wrapped = true; }
+    }
+};
+
+__device__ __forceinline__ uint64_t make_smem_desc(uint32_t addr, int swb) {
+    // K-major, swizzled canonical layout: rows of `swb` bytes, 8-row groups `8*swb`
+    // bytes apart (SBO), LBO = 16 bytes (unused for swizzled K-major), version 1.
+    const uint64_t layout = swb == 128 ? 2ull : (swb == 64 ? 4ull : 6ull);
+    uint64_t d = 0;
+    d |= (uint64_t)((addr & 0x3FFFF) >> 4);
+    d |= (uint64_t)1 << 16;                         // LBO = 16 B
+    d |= (uint64_t)((8 * swb) >> 4) << 32;          // SBO
+    d |= (uint64_t)1 << 46;                         // descriptor version (sm100)
+    d |= layout << 61;
+    return d;
+}
+
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1,
+                                            int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+
+__device__ __forceinline__ void umma_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
+                 ::"r"(smem_u32(bar)) : "memory");
+}
+
+// 16 consecutive fp32 columns of this thread's TMEM lane; no wait (tmem_wait_ld).
+__device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+}  // namespace pb
