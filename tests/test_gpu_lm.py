@@ -392,6 +392,16 @@ def test_sample_settings(vocab, dtype):
                  p=[s.get("p", 1.0) for s in SETTINGS], m=[s.get("m", 0.0) for s in SETTINGS])
 
 
+@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 409600), (torch.float32, 409701), (torch.bfloat16, 900001)])
+def test_sample_long_rows(dtype, vocab):
+    """Rows that do not fit the shared memory of a cluster."""
+    g = gen(vocab)
+    x, e = logits_of(g, 4, vocab, dtype), noise_of(g, 4, vocab)
+    x[3] = -float("inf")
+    tok, _ = check_sample(x, e, t=[0.8, 0.0, 1.5, 1.0], k=[60, 0, 0, 0], p=[0.9, 1.0, 0.97, 1.0])
+    assert tok[1] == x[1].argmax() and tok[3] == -1
+
+
 @pytest.mark.parametrize("rows", [1, 2, 5, 40, 147, 300])
 @pytest.mark.parametrize("vocab", [640, 20011])
 def test_sample_row_counts(rows, vocab):
