@@ -19,6 +19,7 @@
 // winner. The same counting pass also tests the midpoint between the last position
 // known to be kept and `hi`, so rounds are bounded by the bits of a position whatever
 // the variates are; with random ones there are one or two.
+#include <algorithm>
 #include <cuda_fp16.h>
 
 #include "common.h"
@@ -210,36 +211,37 @@ sample_rows_kernel(SampleArgs a, int shift) {
 // A cluster per row: the row is read once, kept in the CTAs' shared memory, and every
 // further pass reads it there.
 // ---------------------------------------------------------------------------
-constexpr int kSlice = 256;             // threads of a CTA
+constexpr int kSlice = 512;             // threads of a CTA
+constexpr int kResident = 2;            // CTAs an SM
 constexpr int kWarps = kSlice / 32;
 constexpr int kBins = 256;
+constexpr int kList = 512;              // candidates that are listed at most (one thread each, at least)
+constexpr int kMostCtas = 8;
 constexpr float kBinsPerOctave = 16.0f; // the bins cover w from 1 down to 2^-16
 
 template <typename T> constexpr int kVec = 16 / (int)sizeof(T);
 template <typename T> constexpr bool kIsHalf = false;
 template <> constexpr bool kIsHalf<__half> = true;
 
-// 16 bytes of logits -> NaN replaced by -inf
-template <typename T> __device__ __forceinline__ uint4 clean_vec(uint4 v);
-template <> __device__ __forceinline__ uint4 clean_vec<float>(uint4 v) {
-    uint32_t* w = &v.x;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(fmaxf(__uint_as_float(w[i]), -INFINITY));
-    return v;
+// A vector of -inf, and the larger of two vectors element by element (a NaN gives way).
+template <typename T> __device__ __forceinline__ uint4 vec_none() {
+    const uint32_t w = sizeof(T) == 4 ? 0xFF800000u : kIsHalf<T> ? 0xFC00FC00u : 0xFF80FF80u;
+    return make_uint4(w, w, w, w);
 }
-template <> __device__ __forceinline__ uint4 clean_vec<__half>(uint4 v) {
-    const __half2 low = __half2half2(__ushort_as_half(0xFC00));
-    __half2* w = reinterpret_cast<__half2*>(&v);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = __hmax2(w[i], low);
-    return v;
+template <typename T> __device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b);
+template <> __device__ __forceinline__ uint32_t word_max<float>(uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
 }
-template <> __device__ __forceinline__ uint4 clean_vec<__nv_bfloat16>(uint4 v) {
-    const __nv_bfloat162 low = __bfloat162bfloat162(__ushort_as_bfloat16(0xFF80));
-    __nv_bfloat162* w = reinterpret_cast<__nv_bfloat162*>(&v);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = __hmax2(w[i], low);
-    return v;
+template <> __device__ __forceinline__ uint32_t word_max<__half>(uint32_t a, uint32_t b) {
+    const __half2 m = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+}
+template <> __device__ __forceinline__ uint32_t word_max<__nv_bfloat16>(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+}
+template <typename T> __device__ __forceinline__ uint4 vec_max_of(const uint4& a, const uint4& b) {
+    return make_uint4(word_max<T>(a.x, b.x), word_max<T>(a.y, b.y), word_max<T>(a.z, b.z), word_max<T>(a.w, b.w));
 }
 template <typename T> __device__ __forceinline__ void unpack(const uint4& v, float (&x)[kVec<T>]);
 template <> __device__ __forceinline__ void unpack<float>(const uint4& v, float (&x)[4]) {
@@ -263,12 +265,11 @@ template <> __device__ __forceinline__ void unpack<__nv_bfloat16>(const uint4& v
     }
 }
 template <typename T> __device__ __forceinline__ float vec_max(const uint4& v) {
+    const uint32_t m = word_max<T>(word_max<T>(v.x, v.y), word_max<T>(v.z, v.w));
+    if (sizeof(T) == 4) return __uint_as_float(m);
     float x[kVec<T>];
-    unpack<T>(v, x);
-    float m = x[0];
-#pragma unroll
-    for (int i = 1; i < kVec<T>; ++i) m = fmaxf(m, x[i]);
-    return m;
+    unpack<T>(make_uint4(m, m, m, m), x);
+    return fmaxf(x[0], x[1]);
 }
 
 // Vectors of a row that may start anywhere: one aligned load, or two and a shift by the
@@ -285,10 +286,10 @@ struct RowLoader {
         words = (int)(off >> 2);
         bits = (int)(off & 3) * 8;
     }
+    // vectors before this one are aligned and whole
+    __device__ __forceinline__ uint32_t easy() const { return (words | bits) == 0 ? n / kVec<T> : 0; }
     __device__ __forceinline__ uint4 operator()(uint32_t v) const {
         const uint32_t i = v * kVec<T>;
-        const bool whole = i + kVec<T> <= n;
-        if ((words | bits) == 0 && whole) return __ldg(base + v);
         // the two vectors lie inside the row unless v is its first or its last
         if (v > 0 && i + 2 * kVec<T> <= n) {
             const uint4 lo = __ldg(base + v), hi = __ldg(base + v + 1);
@@ -323,35 +324,11 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// What the CTAs of a cluster tell each other; one field per kind of join.
-struct Word {
-    float sum0, sum1;           // added
-    int n0, n1;                 // added
-    float key, x;               // a race
-    uint32_t idx;
-    uint32_t least;             // minimum
-};
-
-__device__ __forceinline__ Word word_none() { return Word{0.0f, 0.0f, 0, 0, -1.0f, 0.0f, 0xFFFFFFFFu, 0xFFFFFFFFu}; }
-
-// Joins `w` over lanes `width` apart and less; every lane gets the result.
-__device__ __forceinline__ Word warp_join(Word w, int width) {
-    for (int o = width >> 1; o; o >>= 1) {
-        w.sum0 += __shfl_xor_sync(~0u, w.sum0, o);
-        w.sum1 += __shfl_xor_sync(~0u, w.sum1, o);
-        w.n0 += __shfl_xor_sync(~0u, w.n0, o);
-        w.n1 += __shfl_xor_sync(~0u, w.n1, o);
-        const float k = __shfl_xor_sync(~0u, w.key, o), x = __shfl_xor_sync(~0u, w.x, o);
-        const uint32_t i = __shfl_xor_sync(~0u, w.idx, o);
-        if (k > w.key || (k == w.key && i < w.idx)) { w.key = k; w.idx = i; w.x = x; }
-        w.least = min(w.least, __shfl_xor_sync(~0u, w.least, o));
-    }
-    return w;
-}
-
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_arrive();
+    cluster_wait();
 }
 __device__ __forceinline__ uint32_t remote_u32(const void* p, uint32_t rank) {
     uint32_t v;
@@ -359,44 +336,156 @@ __device__ __forceinline__ uint32_t remote_u32(const void* p, uint32_t rank) {
                  : "=r"(v) : "r"(smem_u32(p)), "r"(rank) : "memory");
     return v;
 }
+__device__ __forceinline__ void remote_store(void* p, uint32_t rank, uint4 v) {
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, %1;\n\tst.shared::cluster.v4.u32 [a], {%2, %3, %4, %5};\n\t}"
+                 ::"r"(smem_u32(p)), "r"(rank), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void remote_store(void* p, uint32_t rank, uint2 v) {
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, %1;\n\tst.shared::cluster.v2.u32 [a], {%2, %3};\n\t}"
+                 ::"r"(smem_u32(p)), "r"(rank), "r"(v.x), "r"(v.y) : "memory");
+}
+
+// The warp-wide joins, over the four words that CTAs tell each other. Whole numbers and
+// the race go through the integer reduction instruction; the order of float sums is fixed.
+struct JoinMax {                // x: a float's bits
+    static __device__ __forceinline__ uint4 none() { return make_uint4(__float_as_uint(-INFINITY), 0, 0, 0); }
+    static __device__ __forceinline__ uint4 warp(uint4 w) {
+        int i = (int)w.x;
+        i ^= (i >> 31) & 0x7FFFFFFF;            // orders as the float does
+        i = __reduce_max_sync(~0u, i);
+        i ^= (i >> 31) & 0x7FFFFFFF;
+        w.x = (uint32_t)i;
+        return w;
+    }
+};
+__device__ __forceinline__ uint32_t warp_sum(uint32_t bits) {
+    float v = __uint_as_float(bits);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+    return __float_as_uint(v);
+}
+struct JoinRace {               // x: the race's key + 1 (0: nobody), y: token, z: its logit's bits, w: mass
+    static __device__ __forceinline__ uint4 none() { return make_uint4(0, 0xFFFFFFFFu, 0, 0); }
+    static __device__ __forceinline__ uint4 warp(uint4 w) {
+        const uint32_t key = __reduce_max_sync(~0u, w.x);
+        const uint32_t idx = w.x == key ? w.y : 0xFFFFFFFFu;
+        const uint32_t best = __reduce_min_sync(~0u, idx);
+        const int from = __ffs(__ballot_sync(~0u, idx == best)) - 1;
+        return make_uint4(key, best, __shfl_sync(~0u, w.z, from), warp_sum(w.w));
+    }
+};
+struct JoinCounts {             // x, y: tokens, z, w: masses
+    static __device__ __forceinline__ uint4 none() { return make_uint4(0, 0, 0, 0); }
+    static __device__ __forceinline__ uint4 warp(uint4 w) {
+        return make_uint4(__reduce_add_sync(~0u, w.x), __reduce_add_sync(~0u, w.y), warp_sum(w.z), warp_sum(w.w));
+    }
+};
+struct JoinLeast {              // x: a token
+    static __device__ __forceinline__ uint4 none() { return make_uint4(0xFFFFFFFFu, 0, 0, 0); }
+    static __device__ __forceinline__ uint4 warp(uint4 w) {
+        w.x = __reduce_min_sync(~0u, w.x);
+        return w;
+    }
+};
+struct JoinList {               // x: candidates, y: most of a CTA, w: mass
+    static __device__ __forceinline__ uint4 none() { return make_uint4(0, 0, 0, 0); }
+    static __device__ __forceinline__ uint4 warp(uint4 w) {
+        return make_uint4(__reduce_add_sync(~0u, w.x), __reduce_max_sync(~0u, w.y), 0, warp_sum(w.w));
+    }
+};
 
 struct Shared {
-    Word part[kWarps];
-    Word told[2];               // this CTA's word of the last two joins
-    uint32_t hist[kBins];
+    uint4 part[kWarps];
+    uint4 told[2][kMostCtas];   // every CTA's word of the last two joins
+    uint2 mine[kList];          // this CTA's candidates: logit, token
+    union {
+        uint32_t hist[kBins];   // tokens per bin of w
+        uint2 list[kList];      // CTA 0: the row's candidates, kList / CTAs places for each
+    };
     uint32_t count[kBins];      // tokens of bins <= b, over the row
     float most[kBins];          // upper bound of their mass
-    float scan[3][kWarps];
+    float scan[3][kBins / 32];
+    uint32_t listed;            // candidates of this CTA, kept or not
+    uint32_t first;
     int cut;
 };
 
-// One join over the cluster. Two slots suffice: a CTA writes a slot again only after the
-// next join's barrier, which every CTA reaches after it has read this one.
-__device__ __forceinline__ Word cluster_join(Word w, Shared& sh, int& turn, int ctas) {
+// One join over the cluster: every CTA's word goes to every other, and every thread gets
+// the result. Two slots suffice: a CTA writes a slot again only after the next join's
+// barrier, which every CTA reaches after it has read this one.
+template <typename J>
+__device__ __forceinline__ uint4 cluster_join(uint4 w, Shared& sh, int& turn, int ctas, uint32_t rank) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    w = warp_join(w, 32);
+    w = J::warp(w);
     if (lane == 0) sh.part[warp] = w;
     __syncthreads();
     if (warp == 0) {
-        w = lane < kWarps ? sh.part[lane] : word_none();
-        w = warp_join(w, 32);
-        if (lane == 0) sh.told[turn] = w;
+        w = J::warp(lane < kWarps ? sh.part[lane] : J::none());
+        if (lane < ctas) remote_store(&sh.told[turn][rank], (uint32_t)lane, w);
         __syncwarp();
     }
     cluster_barrier();
-    Word r = word_none();
-    if (lane < ctas) {
-        const uint32_t* src = reinterpret_cast<const uint32_t*>(&sh.told[turn]);
-        uint32_t* dst = reinterpret_cast<uint32_t*>(&r);
-#pragma unroll
-        for (int i = 0; i < (int)(sizeof(Word) / 4); ++i) dst[i] = remote_u32(src + i, (uint32_t)lane);
-    }
+    w = lane < ctas ? sh.told[turn][lane] : J::none();
     turn ^= 1;
-    return warp_join(r, 32);
+    return J::warp(w);
+}
+
+// The row's token from its candidates (all tokens that can be kept are among the n of
+// them, and those before them in the order), by CTA 0 alone: each candidate counts the
+// candidates and the mass before it. Masses are whole numbers, so that the order in
+// which the list was filled does not matter. If no kept token has a usable variate the
+// first one is the answer. The slice is not needed any more: positions and masses (w * 2^40)
+// lie over it.
+__device__ __forceinline__ uint4 choose(Shared& sh, uint64_t* at_of, int n, int turn, int ctas, int k, bool by_mass, float limit, float top,
+                                        float c, const float* noise, int shift) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int room = kList / ctas;
+    uint64_t* const mass_of = at_of + kList;
+    if (tid < n) {
+        int r = 0, slot = tid;
+        while (slot >= (int)sh.told[turn][r].x) slot -= (int)sh.told[turn][r++].x;
+        const uint2 e = sh.list[r * room + slot];
+        const float x = __uint_as_float(e.x);
+        sh.mine[tid] = e;
+        at_of[tid] = position(x + 0.0f, e.y, shift);
+        mass_of[tid] = (uint64_t)(ex2((x - top) * c) * 1099511627776.0f);
+    }
+    __syncthreads();
+    int g = 1;                              // threads per candidate
+    while (g < 32 && n * g * 2 <= kSlice) g *= 2;
+    const int i = tid / g;
+    uint4 race = JoinRace::none();
+    float e = -1.0f;
+    uint2 own = make_uint2(0, 0);
+    if (i < n) {
+        own = sh.mine[i];
+        if (tid % g == 0) e = __ldg(noise + own.y);
+    }
+    const uint64_t at = i < n ? at_of[i] : 0;
+    uint32_t before = 0;
+    unsigned long long mass = 0;
+    for (int j = tid % g; j < n; j += g)
+        if (at_of[j] < at) { ++before; mass += mass_of[j]; }
+    for (int o = g >> 1; o; o >>= 1) {
+        before += __shfl_xor_sync(~0u, before, o);
+        mass += __shfl_xor_sync(~0u, mass, o);
+    }
+    if (i < n && tid % g == 0) {
+        if (before == 0) sh.first = own.y;
+        const bool kept = before == 0 || ((int)before < k && (!by_mass || (double)mass < (double)limit * 1099511627776.0));
+        if (kept && e >= 0.0f)
+            race = make_uint4(__float_as_uint(__fdividef(ex2((__uint_as_float(own.x) - top) * c), e)) + 1, own.y, own.x, 0);
+    }
+    race = JoinRace::warp(race);
+    if (lane == 0) sh.part[warp] = race;
+    __syncthreads();
+    race = JoinRace::warp(lane < kWarps ? sh.part[lane] : JoinRace::none());
+    if (!race.x) { race.y = sh.first; race.z = __float_as_uint(top); }
+    return race;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kSlice, 4)
+__global__ void __launch_bounds__(kSlice, kResident)
 sample_cluster_kernel(SampleArgs a, int shift, int ctas) {
     constexpr int VEC = kVec<T>;
     extern __shared__ uint4 slice[];
@@ -411,8 +500,9 @@ sample_cluster_kernel(SampleArgs a, int shift, int ctas) {
     float temp = a.temperature ? a.temperature[row] : 1.0f;
     int k = a.top_k ? a.top_k[row] : 0;
     const float p = a.top_p ? a.top_p[row] : 1.0f;
-    const float floor_w = a.min_p ? a.min_p[row] : 0.0f;
+    float floor_w = a.min_p ? a.min_p[row] : 0.0f;
     if (!(temp > 0.0f)) { temp = 1.0f; k = 1; }
+    if (floor_w != floor_w) floor_w = INFINITY;         // no w reaches it
     const bool by_count = k > 0, by_mass = !(p >= 1.0f);
     if (!by_count) k = 0x7FFFFFFF;
 
@@ -420,244 +510,309 @@ sample_cluster_kernel(SampleArgs a, int shift, int ctas) {
     // starts in memory, so that sums do not depend on that.
     const uint32_t nv = (V + VEC - 1) / VEC;
     const uint32_t v0 = (uint32_t)((uint64_t)nv * rank / ctas), all = (uint32_t)((uint64_t)nv * (rank + 1) / ctas) - v0;
-    auto index_of = [&](uint32_t v) { return (v0 + v) * VEC; };
+    const uint32_t i_own = v0 * VEC + tid * VEC;        // first element of this thread's first vector
 
+    cluster_arrive();                   // answered below: before memory of another CTA is written, it has started
     const RowLoader<T> load(lg, V);
-    float mx = -INFINITY;
-    uint32_t at_max = 0;
-#pragma unroll 4
-    for (uint32_t v = tid; v < all; v += kSlice) {
-        const uint4 q = clean_vec<T>(load(v0 + v));
-        slice[v] = q;
-        const float m = vec_max<T>(q);
-        if (m > mx) { mx = m; at_max = v; }
-    }
-    for (int b = tid; b < kBins; b += kSlice) sh.hist[b] = 0;
-    int turn = 0;
-    float tmax = mx;
+    float top;
     {
-        // maximum over the cluster
-        const int warp = tid >> 5, lane = tid & 31;
+        uint4 m = vec_none<T>();
+        const uint32_t easy = min(all, max(load.easy(), v0) - v0);
+        const uint4* src = load.base + v0;
+        auto put = [&](uint32_t v, uint4 q) {
+            q = vec_max_of<T>(q, vec_none<T>());        // NaN -> -inf
+            slice[v] = q;
+            m = vec_max_of<T>(m, q);
+        };
+        uint32_t v = tid;
+        for (; v + 7 * kSlice < easy; v += 8 * kSlice) {
+            uint4 q[8];
 #pragma unroll
-        for (int o = 16; o; o >>= 1) tmax = fmaxf(tmax, __shfl_xor_sync(~0u, tmax, o));
-        if (lane == 0) sh.part[warp].x = tmax;
-        __syncthreads();
-        if (tid == 0) {
-            for (int i = 1; i < kWarps; ++i) tmax = fmaxf(tmax, sh.part[i].x);
-            sh.told[turn].x = tmax;
+            for (int i = 0; i < 8; ++i) q[i] = __ldg(src + v + i * kSlice);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) put(v + i * kSlice, q[i]);
         }
-        __syncwarp();
-        cluster_barrier();
-        tmax = lane < ctas ? __uint_as_float(remote_u32(&sh.told[turn].x, (uint32_t)lane)) : -INFINITY;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) tmax = fmaxf(tmax, __shfl_xor_sync(~0u, tmax, o));
-        turn ^= 1;
+#pragma unroll 4
+        for (; v < easy; v += kSlice) put(v, __ldg(src + v));
+#pragma unroll 2
+        for (; v < all; v += kSlice) put(v, load(v0 + v));
+        for (int b = tid; b < kBins; b += kSlice) sh.hist[b] = 0;
+        if (tid == 0) sh.listed = 0;
+        top = vec_max<T>(m) + 0.0f;
     }
-    const float top = tmax + 0.0f;      // the row's largest logit
-    if (top == -INFINITY) {
+    int turn = 0;
+    cluster_wait();
+    top = __uint_as_float(cluster_join<JoinMax>(make_uint4(__float_as_uint(top), 0, 0, 0), sh, turn, ctas, rank).x);
+    if (top == -INFINITY) {             // nothing to choose from
         if (rank == 0 && tid == 0) {
             a.tokens[row] = -1;
             if (a.probs) a.probs[row] = 0.0f;
         }
-        cluster_barrier();              // no CTA leaves while another may read its memory
         return;
     }
+    if (top == INFINITY) {              // infinite logits share the mass: 0 for them, -inf for the rest
+        for (uint32_t v = tid; v < all; v += kSlice) {
+            uint4 q = slice[v];
+            T* e = reinterpret_cast<T*>(&q);
+            for (int j = 0; j < VEC; ++j) e[j] = logit<T>(e[j]) == INFINITY ? T(0.0f) : T(-INFINITY);
+            slice[v] = q;
+        }
+        top = 0.0f;
+    }
 
-    // w = 2^y with y = (x - top) * log2(e) / T. The clamps keep two products from becoming
-    // NaN: inf - inf (the top itself, y = 0) and -inf * 0 (an infinite temperature).
+    // w = 2^y with y = (x - top) * log2(e) / T; the bound on the factor keeps -inf * 0 out
+    // (an infinite temperature).
     const float c = fmaxf(kLog2e / temp, 1.17549435e-38f);
-    auto exponent = [&](float x) { return fminf((x - top) * c, 0.0f); };
-
-    // Which tokens can be kept? With a min_p that cuts at 2^-6 or above, those it leaves, and
-    // they race in this pass; with no filter at all, every token. Otherwise count the tokens in
-    // bins of w, to find how far down the order the filters can reach.
-    const bool filtered = by_count || by_mass || floor_w > 0.0f;
-    const bool greedy = k == 1;
-    const bool race_now = !greedy && (!filtered || floor_w >= 0.015625f);
-    const bool count_now = !greedy && !race_now;
-    Word w = word_none();
-    float z = 0.0f;
-    Race race;
-    auto enter = [&](float x, uint32_t i, float wx) {
-        const float e = __ldg(noise + i);
-        if (e >= 0.0f && wx > 0.0f) race.take(__fdividef(wx, e), i, x);
+    auto weight = [&](float x) { return ex2((x - top) * c); };
+    auto finish = [&](uint32_t token, float x, float z) {
+        a.tokens[row] = (int32_t)token;
+        if (a.probs) a.probs[row] = (x == top ? 1.0f : expf((x - top) / temp)) / z;
     };
-    for (uint32_t v = tid; v < all; v += kSlice) {
-        float x[VEC], y[VEC], wx[VEC];
-        unpack<T>(slice[v], x);
-        float zz = 0.0f;
+
+    // What the pass that sums Z does beside it:
+    //   race   no filter: every token races
+    //   list   a min_p that cuts at 2^-6 or above: the tokens that it leaves are listed
+    //   count  other filters: tokens are counted in bins of w, to find how far down the
+    //          order the filters can reach
+    //   first  temperature 0: the lowest index of the largest logit
+    enum { kRace, kListing, kCount, kFirst };
+    const int mode = k == 1 ? kFirst : floor_w >= 0.015625f ? kListing : by_count || by_mass || floor_w > 0.0f ? kCount : kRace;
+    const float least_w = fmaxf(floor_w, 1.17549435e-38f);     // of the tokens that race (w > 0)
+    uint4 race = JoinRace::none();
+    // the race of one vector's tokens: all their variates are requested before the first is used
+    auto enter = [&](const float (&x)[VEC], const float (&wx)[VEC], uint32_t i0) {
+        float e[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) e[j] = wx[j] >= least_w ? __ldg(noise + i0 + j) : -1.0f;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            y[j] = exponent(x[j]);
-            wx[j] = ex2(y[j]);
-            zz += wx[j];
+            if (!(e[j] >= 0.0f)) continue;
+            const uint32_t key = __float_as_uint(__fdividef(wx[j], e[j])) + 1;
+            if (key > race.x || (key == race.x && i0 + j < race.y)) { race.x = key; race.y = i0 + j; race.z = __float_as_uint(x[j]); }
         }
-        z += zz;
-        if (race_now) {
+    };
+    auto list = [&](float x, uint32_t i) {
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(noise + i));      // CTA 0 wants it soon
+        const uint32_t slot = atomicAdd(&sh.listed, 1u);
+        if (slot < kList) sh.mine[slot] = make_uint2(__float_as_uint(x), i);
+    };
+    float z = 0.0f;
+    uint32_t first = 0xFFFFFFFFu;
+    for (uint32_t v = tid, i0 = i_own; v < all; v += kSlice, i0 += kSlice * VEC) {
+        float x[VEC], wx[VEC];
+        unpack<T>(slice[v], x);
+        float2 zz = make_float2(0.0f, 0.0f);
+        float2 y[VEC / 2];
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+            y[j / 2] = __fmul2_rn(__fadd2_rn(make_float2(x[j], x[j + 1]), make_float2(-top, -top)), make_float2(c, c));
+            wx[j] = ex2(y[j / 2].x);
+            wx[j + 1] = ex2(y[j / 2].y);
+            zz = __fadd2_rn(zz, make_float2(wx[j], wx[j + 1]));
+        }
+        z += zz.x + zz.y;
+        if (mode == kListing) {
             float m = wx[0];
 #pragma unroll
             for (int j = 1; j < VEC; ++j) m = fmaxf(m, wx[j]);
-            if (m >= floor_w) {
-                const uint32_t i0 = index_of(v);
+            if (m >= least_w) {
 #pragma unroll
                 for (int j = 0; j < VEC; ++j)
-                    if (wx[j] >= floor_w && x[j] > -INFINITY) enter(x[j], i0 + j, wx[j]);
+                    if (wx[j] >= least_w) list(x[j], i0 + j);
             }
-        } else if (count_now) {
+        } else if (mode == kCount) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                const float t = y[j] * -kBinsPerOctave;
+                const float t = (j & 1 ? y[j / 2].y : y[j / 2].x) * -kBinsPerOctave;
                 if (t < (float)kBins) atomicAdd(&sh.hist[(int)t], 1u);
             }
-        }
-    }
-    w.sum0 = z;
-    w.key = race.key; w.idx = race.idx; w.x = race.x;
-    // lowest index of the largest logit
-    if (mx == top) {
-        float x[VEC];
-        unpack<T>(slice[at_max], x);
-        for (int j = VEC - 1; j >= 0; --j)
-            if (x[j] == top) w.least = index_of(at_max) + j;
-    }
-    w = cluster_join(w, sh, turn, ctas);
-    z = w.sum0;
-    const uint32_t first = w.least;
-    const float limit = p * z;
-    Race won;
-    won.key = w.key; won.idx = w.idx; won.x = w.x;
-
-    bool done = greedy || (race_now && !by_count && !by_mass);
-    if (greedy) won.idx = 0xFFFFFFFFu;      // the first token
-    uint64_t lo = position(top, first, shift), hi = position(-INFINITY, 0, shift);
-    bool have = race_now;
-    if (count_now) {
-        // bin b holds tokens with w in (2^(-(b + 1) / 16), 2^(-b / 16)]
-        const int warp = tid >> 5, lane = tid & 31;
-        uint32_t n = 0;
-        for (int r = 0; r < ctas; ++r) n += remote_u32(&sh.hist[tid], (uint32_t)r);
-        float least = (float)n * ex2(-(float)(tid + 1) / kBinsPerOctave);
-        float most = (float)n * ex2(-(float)tid / kBinsPerOctave);
-        float cnt = (float)n;               // exact: at most 2^24 matter, and more only say "many"
+        } else if (mode == kRace) {
+            enter(x, wx, i0);
+        } else if (first == 0xFFFFFFFFu) {
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const float c1 = __shfl_up_sync(~0u, cnt, o), l1 = __shfl_up_sync(~0u, least, o), m1 = __shfl_up_sync(~0u, most, o);
-            if (lane >= o) { cnt += c1; least += l1; most += m1; }
+            for (int j = VEC - 1; j >= 0; --j)
+                if (x[j] == top) first = i0 + j;
         }
-        if (lane == 31) { sh.scan[0][warp] = cnt; sh.scan[1][warp] = least; sh.scan[2][warp] = most; }
-        if (tid == 0) sh.cut = kBins;
+    }
+
+    const int room = kList / ctas;
+    // this CTA's candidates to CTA 0; call with every thread, then join
+    auto send = [&]() {
         __syncthreads();
-        for (int i = 0; i < warp; ++i) { cnt += sh.scan[0][i]; least += sh.scan[1][i]; most += sh.scan[2][i]; }
-        sh.count[tid] = (uint32_t)fminf(cnt, 2147483520.0f);
-        sh.most[tid] = most;
-        // every kept token is in this bin or one before it
-        if ((by_count && cnt >= (float)k) || (by_mass && least >= limit * 1.0001f)) atomicMin(&sh.cut, tid);
+        const uint32_t n = min(sh.listed, (uint32_t)room);
+        for (uint32_t i = tid; i < n; i += kSlice) remote_store(&sh.list[rank * room + i], 0u, sh.mine[i]);
+    };
+    uint4 won = JoinRace::none();
+    bool done = false, have = false;
+    float limit;
+    if (mode == kListing) {
+        send();
+        const uint4 w = cluster_join<JoinList>(make_uint4(tid ? 0 : sh.listed, tid ? 0 : sh.listed, 0, __float_as_uint(z)), sh, turn, ctas, rank);
+        z = __uint_as_float(w.w);
+        limit = p * z;
+        if (w.x && w.y <= (uint32_t)room) {
+            if (rank) return;
+            won = choose(sh, reinterpret_cast<uint64_t*>(slice), (int)w.x, turn ^ 1, ctas, k, by_mass, limit, top, c, noise, shift);
+            if (tid == 0) finish(won.y, __uint_as_float(won.z), z);
+            return;
+        }
+        done = !w.x;            // min_p above 1: the first token
+    } else {
+        race.w = __float_as_uint(z);
+        won = cluster_join<JoinRace>(race, sh, turn, ctas, rank);
+        z = __uint_as_float(won.w);
+        limit = p * z;
+        done = mode != kCount;
+    }
+    if (mode == kCount) {
+        // bin b holds tokens with w in (2^-((b + 1) / 16), 2^-(b / 16)]
+        const int warp = tid >> 5, lane = tid & 31;
+        float cnt = 0.0f, least = 0.0f, most = 0.0f;
+        if (tid == 0) sh.cut = kBins;
+        if (tid < kBins) {
+            uint32_t n = 0;
+            for (int r = 0; r < ctas; ++r) n += remote_u32(&sh.hist[tid], (uint32_t)r);
+            cnt = (float)n;     // exact up to 2^24 tokens, more than the slices can hold
+            least = cnt * ex2(-(float)(tid + 1) / kBinsPerOctave);
+            most = cnt * ex2(-(float)tid / kBinsPerOctave);
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const float c1 = __shfl_up_sync(~0u, cnt, o), l1 = __shfl_up_sync(~0u, least, o), m1 = __shfl_up_sync(~0u, most, o);
+                if (lane >= o) { cnt += c1; least += l1; most += m1; }
+            }
+            if (lane == 31) { sh.scan[0][warp] = cnt; sh.scan[1][warp] = least; sh.scan[2][warp] = most; }
+        }
+        __syncthreads();
+        if (tid < kBins) {
+            for (int i = 0; i < warp; ++i) { cnt += sh.scan[0][i]; least += sh.scan[1][i]; most += sh.scan[2][i]; }
+            sh.count[tid] = (uint32_t)cnt;
+            sh.most[tid] = most;
+            // every kept token is in this bin or one before it
+            if ((by_count && cnt >= (float)k) || (by_mass && least >= limit * 1.0001f)) atomicMin(&sh.cut, tid);
+        }
         __syncthreads();
         const int cut = sh.cut;
-        // logits of the bins up to the cut, a little below to be safe against rounding
+        // logits of the bins up to the cut, from a little below to be safe against rounding
         float from = -INFINITY;
         if (cut < kBins) {
             from = top - ((float)(cut + 1) / kBinsPerOctave) / c;
-            if (top < INFINITY) from -= 1e-5f * (fabsf(top) + fabsf(from)) + 1e-5f / c;
+            from -= 1e-5f * (fabsf(top) + fabsf(from)) + 1e-5f / c;
         }
-        race = Race();
-        for (uint32_t v = tid; v < all; v += kSlice) {
+        // few enough to be listed (the margin may add some: then they do not all fit and the
+        // race below goes on)
+        const bool few = cut < kBins && sh.count[cut] <= (uint32_t)kList;
+        if (few) cluster_barrier();     // the histograms have been read: CTA 0's list takes their place
+        for (uint32_t v = tid, i0 = i_own; v < all; v += kSlice, i0 += kSlice * VEC) {
             const uint4 q = slice[v];
             if (!(vec_max<T>(q) >= from)) continue;
-            float x[VEC];
+            float x[VEC], wx[VEC];
             unpack<T>(q, x);
-            const uint32_t i0 = index_of(v);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                if (!(x[j] >= from) || x[j] == -INFINITY) continue;
-                const float wx = ex2(exponent(x[j]));
-                if (wx >= floor_w) enter(x[j], i0 + j, wx);
+                wx[j] = x[j] >= from ? weight(x[j]) : 0.0f;
+                if (few && wx[j] >= least_w) list(x[j], i0 + j);
             }
+            if (!few) enter(x, wx, i0);
         }
-        w = word_none();
-        w.key = race.key; w.idx = race.idx; w.x = race.x;
-        w = cluster_join(w, sh, turn, ctas);
-        won.key = w.key; won.idx = w.idx; won.x = w.x;
-        have = true;
-        // surely kept: even all tokens of its bin and those before are few and light enough
-        if (won.idx != 0xFFFFFFFFu) {
-            const float t = exponent(won.x) * -kBinsPerOctave;
-            if (t < (float)kBins) {
-                const int b = (int)t;
-                if ((!by_count || sh.count[b] <= (uint32_t)k) && (!by_mass || sh.most[b] < limit * 0.9999f)) done = true;
+        if (few) {
+            send();
+            const uint4 w = cluster_join<JoinList>(make_uint4(tid ? 0 : sh.listed, tid ? 0 : sh.listed, 0, 0), sh, turn, ctas, rank);
+            if (w.x && w.y <= (uint32_t)room) {
+                if (rank) return;
+                won = choose(sh, reinterpret_cast<uint64_t*>(slice), (int)w.x, turn ^ 1, ctas, k, by_mass, limit, top, c, noise, shift);
+                if (tid == 0) finish(won.y, __uint_as_float(won.z), z);
+                return;
+            }
+        } else {
+            won = cluster_join<JoinRace>(race, sh, turn, ctas, rank);
+            have = true;
+            // surely kept: even all tokens of its bin and those before are few and light enough
+            if (won.x) {
+                const float t = (__uint_as_float(won.z) - top) * c * -kBinsPerOctave;
+                if (t < (float)kBins) {
+                    const int b = (int)t;
+                    done = (!by_count || sh.count[b] <= (uint32_t)k) && (!by_mass || sh.most[b] < limit * 0.9999f);
+                }
             }
         }
     }
     // Rounds: is the winner kept? If not, race again before it. From the third round on the
     // midpoint between what is known to be in and to be out is tested too.
+    uint64_t lo = position(top, 0, shift), hi = position(-INFINITY, 0, shift);
     for (int round = 0; !done; ++round) {
         if (!have) {
-            race = Race();
+            race = JoinRace::none();
             const float from = value_of(hi, shift);
-            for (uint32_t v = tid; v < all; v += kSlice) {
+            for (uint32_t v = tid, i0 = i_own; v < all; v += kSlice, i0 += kSlice * VEC) {
                 const uint4 q = slice[v];
                 if (vec_max<T>(q) < from) continue;
-                float x[VEC];
+                float x[VEC], wx[VEC];
                 unpack<T>(q, x);
-                const uint32_t i0 = index_of(v);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    if (x[j] == -INFINITY || position(x[j] + 0.0f, i0 + j, shift) >= hi) continue;
-                    const float wx = ex2(exponent(x[j]));
-                    if (wx >= floor_w) enter(x[j], i0 + j, wx);
-                }
+                for (int j = 0; j < VEC; ++j) wx[j] = position(x[j] + 0.0f, i0 + j, shift) < hi ? weight(x[j]) : 0.0f;
+                enter(x, wx, i0);
             }
-            w = word_none();
-            w.key = race.key; w.idx = race.idx; w.x = race.x;
-            w = cluster_join(w, sh, turn, ctas);
-            won.key = w.key; won.idx = w.idx; won.x = w.x;
+            won = cluster_join<JoinRace>(race, sh, turn, ctas, rank);
         }
         have = false;
-        if (won.idx == 0xFFFFFFFFu) break;
-        const uint64_t at_won = position(won.x + 0.0f, won.idx, shift);
+        if (!won.x) break;
+        const float x_won = __uint_as_float(won.z);
+        const uint64_t at_won = position(x_won + 0.0f, won.y, shift);
         if (at_won <= lo) break;
         const uint64_t mid = round < 2 ? lo : lo + (hi - lo) / 2;
-        const float from = fminf(won.x, value_of(mid, shift));
-        w = word_none();
-        for (uint32_t v = tid; v < all; v += kSlice) {
+        const float from = fminf(x_won, value_of(mid, shift));
+        uint32_t n0 = 0, n1 = 0;
+        float m0 = 0.0f, m1 = 0.0f;
+        for (uint32_t v = tid, i0 = i_own; v < all; v += kSlice, i0 += kSlice * VEC) {
             const uint4 q = slice[v];
             if (vec_max<T>(q) < from) continue;
             float x[VEC];
             unpack<T>(q, x);
-            const uint32_t i0 = index_of(v);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                if (x[j] == -INFINITY) continue;
                 const uint64_t at = position(x[j] + 0.0f, i0 + j, shift);
                 if (at >= at_won && at >= mid) continue;
-                const float wx = ex2(exponent(x[j]));
-                if (at < at_won) { ++w.n0; w.sum0 += wx; }
-                if (at < mid) { ++w.n1; w.sum1 += wx; }
+                const float wx = weight(x[j]);
+                if (at < at_won) { ++n0; m0 += wx; }
+                if (at < mid) { ++n1; m1 += wx; }
             }
         }
-        w = cluster_join(w, sh, turn, ctas);
-        if (w.n0 < k && (!by_mass || w.sum0 < limit)) break;
+        const uint4 w = cluster_join<JoinCounts>(make_uint4(n0, n1, __float_as_uint(m0), __float_as_uint(m1)), sh, turn, ctas, rank);
+        if ((int)w.x < k && (!by_mass || __uint_as_float(w.z) < limit)) break;
         hi = at_won;
         if (round >= 2) {
-            if (w.n1 < k && (!by_mass || w.sum1 < limit)) lo = max(lo, mid);
+            if ((int)w.y < k && (!by_mass || __uint_as_float(w.w) < limit)) lo = max(lo, mid);
             else hi = min(hi, mid);
         }
     }
-    if (rank == 0 && tid == 0) {
-        const bool none = won.idx == 0xFFFFFFFFu;       // no usable variate: the first token
-        a.tokens[row] = (int32_t)(none ? first : won.idx);
-        if (a.probs) a.probs[row] = (none || won.x == top ? 1.0f : expf((won.x - top) / temp)) / z;
+    if (!won.x) {                       // temperature 0, or no usable variate: the first token
+        if (mode != kFirst) {
+            for (uint32_t v = tid, i0 = i_own; v < all && first == 0xFFFFFFFFu; v += kSlice, i0 += kSlice * VEC) {
+                float x[VEC];
+                unpack<T>(slice[v], x);
+#pragma unroll
+                for (int j = VEC - 1; j >= 0; --j)
+                    if (x[j] == top) first = i0 + j;
+            }
+        }
+        won.y = cluster_join<JoinLeast>(make_uint4(first, 0, 0, 0), sh, turn, ctas, rank).x;
+        won.z = __float_as_uint(top);
     }
-    cluster_barrier();
+    if (rank == 0 && tid == 0) finish(won.y, __uint_as_float(won.z), z);
 }
 
 template <typename T>
 bool launch_cluster(const SampleArgs& a, int shift, cudaStream_t s) {
     const int64_t bytes = a.vocab * (int64_t)sizeof(T);
-    constexpr int64_t kMost = 200 * 1024;
-    int ctas = 8;
-    if (bytes / ctas > kMost) return false;
-    const size_t smem = (size_t)(((a.vocab + kVec<T> - 1) / kVec<T> + ctas - 1) / ctas) * 16;
+    constexpr int64_t kMost = 200 * 1024;      // of a slice
+    if (bytes / kMostCtas > kMost) return false;
+    // As many CTAs per row as leave every row's cluster resident at once (two CTAs an SM), but
+    // enough for slices of 64 KB. Measured (us, bf16 unless said): 1 row of 32000: 8 CTAs 6.1, 2 CTAs 7.2;
+    // 33 of 50257 (f32): 8: 16.0, 4: 18.2; 64 of 131072: 4: 15.9, 8: 21.3, 2: 17.0; 128 of 32000 (f32):
+    // 2: 22.0, 4: 24.3; 256 of 131072: 4: 48.6, 2: 54.7, 8: 66.9.
+    const int64_t fit = 2 * 148 / a.rows, need = (bytes + 65535) / 65536;
+    const int ctas = (int)std::min<int64_t>(kMostCtas, std::max(fit, need));
+    const size_t smem = std::max<size_t>((size_t)(((a.vocab + kVec<T> - 1) / kVec<T> + ctas - 1) / ctas) * 16, 2 * kList * 8);
     static bool ready[64] = {};
     int device = 0;
     PB_CUDA(cudaGetDevice(&device));
