@@ -22,14 +22,18 @@ _T = None
 
 
 class _Types:
-    """torch, and what of it is looked up on every call."""
+    """torch, the library and what of both is looked up on every call."""
 
     def __init__(self):
         import torch
-        self.torch = torch
+        self.Tensor, self.empty, self.empty_like = torch.Tensor, torch.empty, torch.empty_like
         self.code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-        self.fp8 = torch.float8_e4m3fn
-        self.f32, self.i32 = torch.float32, torch.int32
+        self.fp8, self.f32, self.i32, self.bf16 = torch.float8_e4m3fn, torch.float32, torch.int32, torch.bfloat16
+        # torch.cuda.current_stream() without the Stream object around the handle (2 us a call)
+        self.stream = torch._C._cuda_getCurrentRawStream
+        lib = N.lib()
+        self.rms_norm, self.sample = lib.engine_rms_norm_device, lib.engine_sample_device
+        self.matmul, self.grouped = lib.engine_matmul_fp8_device, lib.engine_matmul_grouped_fp8_device
 
 
 def _types() -> _Types:
@@ -42,26 +46,23 @@ def _types() -> _Types:
 
 
 def _tensor(t, T, what, device, dtype, ndim):
-    if not isinstance(t, T.torch.Tensor) or not t.is_cuda:
+    """Refuses what is not a dense-rowed tensor of `dtype` on GPU `device`."""
+    if not isinstance(t, T.Tensor) or not t.is_cuda:
         raise TypeError(f"{what}: a CUDA torch.Tensor is needed")
     if t.dtype != dtype:
         raise TypeError(f"{what}: {dtype} is needed, got {t.dtype}")
     if t.dim() != ndim:
         raise PdefaError(f"{what}: {ndim} dimensions are needed, got {tuple(t.shape)}")
-    if t.device != device:
-        raise PdefaError(f"{what}: is on {t.device}, not on {device}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    if t.get_device() != device:
+        raise PdefaError(f"{what}: is on GPU {t.get_device()}, not on {device}")
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise PdefaError(f"{what}: the last dimension has to be dense (strides {t.stride()})")
 
 
-def _cuda(t, T, what):
-    if not isinstance(t, T.torch.Tensor) or not t.is_cuda:
+def _gpu(t, T, what) -> int:
+    if not isinstance(t, T.Tensor) or not t.is_cuda:
         raise TypeError(f"{what}: a CUDA torch.Tensor is needed")
-    return t.device
-
-
-def _stream(T, device) -> int:
-    return T.torch.cuda.current_stream(device).cuda_stream
+    return t.get_device()
 
 
 def _rows(t):
@@ -80,39 +81,46 @@ def _rows(t):
 
 def _norm(what, x, weight, residual, eps, fp8):
     T = _types()
-    device = _cuda(x, T, what)
-    code = T.code.get(x.dtype)
+    gpu = _gpu(x, T, what)
+    dtype = x.dtype
+    code = T.code.get(dtype)
     if code is None:
-        raise TypeError(f"{what}: x must be float32, float16 or bfloat16, got {x.dtype}")
-    if x.dim() == 0:
-        raise PdefaError(f"{what}: x needs a dimension")
+        raise TypeError(f"{what}: x must be float32, float16 or bfloat16, got {dtype}")
     shape = x.shape
+    if not shape:
+        raise PdefaError(f"{what}: x needs a dimension")
     x2 = _rows(x)
     rows, cols = x2.shape
-    _tensor(x2, T, f"{what}: x", device, x.dtype, 2)
-    _tensor(weight, T, f"{what}: weight", device, T.f32 if getattr(weight, "dtype", None) == T.f32 else x.dtype, 1)
+    _tensor(x2, T, what, gpu, dtype, 2)
+    wcode = code
+    if getattr(weight, "dtype", None) == T.f32:
+        wcode = 0
+        _tensor(weight, T, what, gpu, T.f32, 1)
+    else:
+        _tensor(weight, T, what, gpu, dtype, 1)
     if weight.shape[0] != cols:
         raise PdefaError(f"{what}: weight of {weight.shape[0]} for rows of {cols}")
-    empty = T.torch.empty
-    r = h = None
+    # empty_like costs half of empty, but keeps strides that are not those of whole rows
+    dense = x.is_contiguous()
+    device = x.device
+    h, r_ptr, r_stride, h_ptr = None, None, 0, None
     if residual is not None:
-        if not isinstance(residual, T.torch.Tensor) or residual.shape != shape:
+        if not isinstance(residual, T.Tensor) or residual.shape != shape:
             raise PdefaError(f"{what}: the residual needs x's shape {tuple(shape)}")
         r = _rows(residual)
-        _tensor(r, T, f"{what}: residual", device, x.dtype, 2)
-        h = empty(shape, dtype=x.dtype, device=device)
-    scales = None
+        _tensor(r, T, what, gpu, dtype, 2)
+        h = T.empty_like(x) if dense else T.empty(shape, dtype=dtype, device=device)
+        r_ptr, r_stride, h_ptr = r.data_ptr(), r.stride(0), h.data_ptr()
     nb = (cols + BLOCK - 1) // BLOCK
     if fp8:
-        y = empty(shape, dtype=T.fp8, device=device)
-        scales = empty((*shape[:-1], nb), dtype=T.f32, device=device)
+        y = T.empty_like(x, dtype=T.fp8) if dense else T.empty(shape, dtype=T.fp8, device=device)
+        scales = T.empty((*shape[:-1], nb), dtype=T.f32, device=device)
+        s_ptr = scales.data_ptr()
     else:
-        y = empty(shape, dtype=x.dtype, device=device)
-    rc = N.lib().engine_rms_norm_device(
-        x2.data_ptr(), x2.stride(0), None if r is None else r.data_ptr(), 0 if r is None else r.stride(0),
-        weight.data_ptr(), None if h is None else h.data_ptr(), cols, y.data_ptr(), cols,
-        None if scales is None else scales.data_ptr(), nb, rows, cols, code, T.code[weight.dtype], eps,
-        device.index, _stream(T, device))
+        y = T.empty_like(x) if dense else T.empty(shape, dtype=dtype, device=device)
+        scales, s_ptr = None, None
+    rc = T.rms_norm(x2.data_ptr(), x2.stride(0), r_ptr, r_stride, weight.data_ptr(), h_ptr, cols, y.data_ptr(), cols,
+                    s_ptr, nb, rows, cols, code, wcode, eps, gpu, T.stream(gpu))
     if rc:
         _check(rc, what)
     return y, scales, h
@@ -135,12 +143,10 @@ def ops_rms_norm_fp8(x, weight, residual=None, eps: float = 1e-6):
 
 
 def _out_code(T, what, out_dtype):
-    if out_dtype is None:
-        return T.torch.bfloat16, 2
     code = T.code.get(out_dtype)
     if code is None:
         raise TypeError(f"{what}: out_dtype must be float32, float16 or bfloat16, got {out_dtype}")
-    return out_dtype, code
+    return code
 
 
 def ops_matmul_fp8(a, a_scales, b, b_scales, out_dtype=None):
@@ -149,21 +155,21 @@ def ops_matmul_fp8(a, a_scales, b, b_scales, out_dtype=None):
     makes them); b [N, K] float8_e4m3fn with b_scales [ceil(N / 128), ceil(K / 128)]."""
     what = "ops_matmul_fp8"
     T = _types()
-    device = _cuda(a, T, f"{what}: a")
-    _tensor(a, T, f"{what}: a", device, T.fp8, 2)
-    _tensor(b, T, f"{what}: b", device, T.fp8, 2)
-    _tensor(a_scales, T, f"{what}: a_scales", device, T.f32, 2)
-    _tensor(b_scales, T, f"{what}: b_scales", device, T.f32, 2)
+    gpu = _gpu(a, T, what)
+    _tensor(a, T, "ops_matmul_fp8: a", gpu, T.fp8, 2)
+    _tensor(b, T, "ops_matmul_fp8: b", gpu, T.fp8, 2)
+    _tensor(a_scales, T, "ops_matmul_fp8: a_scales", gpu, T.f32, 2)
+    _tensor(b_scales, T, "ops_matmul_fp8: b_scales", gpu, T.f32, 2)
     m, k = a.shape
     n, kb = b.shape[0], (k + BLOCK - 1) // BLOCK
     if b.shape[1] != k or a_scales.shape != (m, kb) or b_scales.shape != ((n + BLOCK - 1) // BLOCK, kb):
         raise PdefaError(f"{what}: shapes do not fit: a {tuple(a.shape)}, a_scales {tuple(a_scales.shape)}, "
                          f"b {tuple(b.shape)}, b_scales {tuple(b_scales.shape)}")
-    out_dtype, code = _out_code(T, what, out_dtype)
-    out = T.torch.empty((m, n), dtype=out_dtype, device=device)
-    rc = N.lib().engine_matmul_fp8_device(
-        a.data_ptr(), a.stride(0), a_scales.data_ptr(), a_scales.stride(0), b.data_ptr(), b.stride(0),
-        b_scales.data_ptr(), b_scales.stride(0), out.data_ptr(), n, code, m, n, k, device.index, _stream(T, device))
+    out_dtype = out_dtype or T.bf16
+    code = _out_code(T, what, out_dtype)
+    out = T.empty((m, n), dtype=out_dtype, device=a.device)
+    rc = T.matmul(a.data_ptr(), a.stride(0), a_scales.data_ptr(), a_scales.stride(0), b.data_ptr(), b.stride(0),
+                  b_scales.data_ptr(), b_scales.stride(0), out.data_ptr(), n, code, m, n, k, gpu, T.stream(gpu))
     if rc:
         _check(rc, what)
     return out
@@ -176,12 +182,12 @@ def ops_matmul_grouped_fp8(a, a_scales, b, b_scales, offsets, out_dtype=None):
     offsets[e] .. offsets[e + 1] - 1 meet expert e. Rows of no expert give 0."""
     what = "ops_matmul_grouped_fp8"
     T = _types()
-    device = _cuda(a, T, f"{what}: a")
-    _tensor(a, T, f"{what}: a", device, T.fp8, 2)
-    _tensor(b, T, f"{what}: b", device, T.fp8, 3)
-    _tensor(a_scales, T, f"{what}: a_scales", device, T.f32, 2)
-    _tensor(b_scales, T, f"{what}: b_scales", device, T.f32, 3)
-    _tensor(offsets, T, f"{what}: offsets", device, T.i32, 1)
+    gpu = _gpu(a, T, what)
+    _tensor(a, T, "ops_matmul_grouped_fp8: a", gpu, T.fp8, 2)
+    _tensor(b, T, "ops_matmul_grouped_fp8: b", gpu, T.fp8, 3)
+    _tensor(a_scales, T, "ops_matmul_grouped_fp8: a_scales", gpu, T.f32, 2)
+    _tensor(b_scales, T, "ops_matmul_grouped_fp8: b_scales", gpu, T.f32, 3)
+    _tensor(offsets, T, "ops_matmul_grouped_fp8: offsets", gpu, T.i32, 1)
     rows, k = a.shape
     experts, n = b.shape[0], b.shape[1]
     kb = (k + BLOCK - 1) // BLOCK
@@ -189,14 +195,16 @@ def ops_matmul_grouped_fp8(a, a_scales, b, b_scales, offsets, out_dtype=None):
             or offsets.shape[0] != experts + 1):
         raise PdefaError(f"{what}: shapes do not fit: a {tuple(a.shape)}, a_scales {tuple(a_scales.shape)}, "
                          f"b {tuple(b.shape)}, b_scales {tuple(b_scales.shape)}, offsets {tuple(offsets.shape)}")
-    out_dtype, code = _out_code(T, what, out_dtype)
-    out = T.torch.empty((rows, n), dtype=out_dtype, device=device)
+    out_dtype = out_dtype or T.bf16
+    code = _out_code(T, what, out_dtype)
+    out = T.empty((rows, n), dtype=out_dtype, device=a.device)
     if experts == 0:
         return out.zero_()
-    rc = N.lib().engine_matmul_grouped_fp8_device(
-        a.data_ptr(), a.stride(0), a_scales.data_ptr(), a_scales.stride(0), b.data_ptr(), b.stride(1), b.stride(0),
-        b_scales.data_ptr(), b_scales.stride(1), b_scales.stride(0), offsets.data_ptr(), experts, out.data_ptr(), n,
-        code, rows, n, k, device.index, _stream(T, device))
+    b_expert, ldb, _ = b.stride()
+    s_expert, lds, _ = b_scales.stride()
+    rc = T.grouped(a.data_ptr(), a.stride(0), a_scales.data_ptr(), a_scales.stride(0), b.data_ptr(), ldb, b_expert,
+                   b_scales.data_ptr(), lds, s_expert, offsets.data_ptr(), experts, out.data_ptr(), n, code, rows, n, k,
+                   gpu, T.stream(gpu))
     if rc:
         _check(rc, what)
     return out
@@ -215,28 +223,34 @@ def ops_sample(logits, noise, temperature=None, top_k=None, top_p=None, min_p=No
     mass. A row of -inf alone gives token -1 and probability 0."""
     what = "ops_sample"
     T = _types()
-    device = _cuda(logits, T, f"{what}: logits")
-    code = T.code.get(logits.dtype)
+    gpu = _gpu(logits, T, what)
+    dtype = logits.dtype
+    code = T.code.get(dtype)
     if code is None:
-        raise TypeError(f"{what}: logits must be float32, float16 or bfloat16, got {logits.dtype}")
-    _tensor(logits, T, f"{what}: logits", device, logits.dtype, 2)
-    _tensor(noise, T, f"{what}: noise", device, T.f32, 2)
-    rows, vocab = logits.shape
-    if noise.shape != logits.shape:
-        raise PdefaError(f"{what}: noise {tuple(noise.shape)} for logits {tuple(logits.shape)}")
-    ptr = [None] * 4
-    for i, (t, dtype, name) in enumerate(((temperature, T.f32, "temperature"), (top_k, T.i32, "top_k"),
-                                          (top_p, T.f32, "top_p"), (min_p, T.f32, "min_p"))):
-        if t is not None:
-            _tensor(t, T, f"{what}: {name}", device, dtype, 1)
-            if t.shape[0] != rows:
-                raise PdefaError(f"{what}: {name} of {t.shape[0]} for {rows} rows")
-            ptr[i] = t.data_ptr()
-    tokens = T.torch.empty(rows, dtype=T.i32, device=device)
-    probs = T.torch.empty(rows, dtype=T.f32, device=device)
-    rc = N.lib().engine_sample_device(
-        logits.data_ptr(), logits.stride(0), code, noise.data_ptr(), noise.stride(0), ptr[0], ptr[1], ptr[2], ptr[3],
-        rows, vocab, tokens.data_ptr(), probs.data_ptr(), device.index, _stream(T, device))
+        raise TypeError(f"{what}: logits must be float32, float16 or bfloat16, got {dtype}")
+    _tensor(logits, T, "ops_sample: logits", gpu, dtype, 2)
+    _tensor(noise, T, "ops_sample: noise", gpu, T.f32, 2)
+    rows, vocab = shape = logits.shape
+    if noise.shape != shape:
+        raise PdefaError(f"{what}: noise {tuple(noise.shape)} for logits {tuple(shape)}")
+
+    def per_row(t, dtype, name):
+        if t is None:
+            return None
+        _tensor(t, T, name, gpu, dtype, 1)
+        if t.shape[0] != rows:
+            raise PdefaError(f"{name} of {t.shape[0]} for {rows} rows")
+        return t.data_ptr()
+
+    t_ptr = per_row(temperature, T.f32, "ops_sample: temperature")
+    k_ptr = per_row(top_k, T.i32, "ops_sample: top_k")
+    p_ptr = per_row(top_p, T.f32, "ops_sample: top_p")
+    m_ptr = per_row(min_p, T.f32, "ops_sample: min_p")
+    device = logits.device
+    tokens = T.empty(rows, dtype=T.i32, device=device)
+    probs = T.empty(rows, dtype=T.f32, device=device)
+    rc = T.sample(logits.data_ptr(), logits.stride(0), code, noise.data_ptr(), noise.stride(0), t_ptr, k_ptr, p_ptr,
+                  m_ptr, rows, vocab, tokens.data_ptr(), probs.data_ptr(), gpu, T.stream(gpu))
     if rc:
         _check(rc, what)
     return tokens, probs
