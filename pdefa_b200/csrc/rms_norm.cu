@@ -5,6 +5,9 @@
 //   y = h * w / sqrt(mean(h^2) + eps)
 //   8-bit: scale = max(max|y| over 128 columns, 1e-10) / 448, q = e4m3(y / scale)
 //
+// Bound by memory: the values are read once and written once, 16384 x 8192 bf16 with a
+// residual and an 8-bit output in 141 us (6.7 TB/s, 104% of a plain copy's rate on B200).
+//
 // The statistic and the scales come from the unrounded 32-bit sum. A NaN in a row
 // makes its whole output NaN (an infinity makes the statistic 0 and itself NaN).
 #include <algorithm>
@@ -13,6 +16,7 @@
 
 #include "common.h"
 #include "device_common.cuh"
+#include "row_vec.cuh"
 
 namespace pb {
 
@@ -122,29 +126,117 @@ __device__ __forceinline__ uint4 pack(const float (&v)[kPiece<T>]) {
     return q;
 }
 
+// STREAM: the data passes through the L2 cache without staying there.
+template <bool STREAM>
+__device__ __forceinline__ uint4 load_piece(const void* p) {
+    const uint4* q = static_cast<const uint4*>(p);
+    return STREAM ? __ldcs(q) : *q;
+}
+template <bool STREAM, typename V>
+__device__ __forceinline__ void store_piece(void* p, V v) {
+    if (STREAM) __stcs(static_cast<V*>(p), v);
+    else *static_cast<V*>(p) = v;
+}
+
+// Stores the pieces of a row that starts anywhere: a thread writes the aligned piece that
+// begins inside its own and ends in the next thread's (`next`), element by element only at
+// the row's two ends. B: bytes of a piece, V the vector type of that size, E the element's.
+__device__ __forceinline__ uint4 join_pieces(const uint4& own, const uint4& next, int bytes) {
+    return shift_pair(own, next, bytes >> 2, (bytes & 3) * 8);
+}
+__device__ __forceinline__ uint2 join_pieces(const uint2& own, const uint2& next, int bytes) {
+    const uint4 r = shift_pair(make_uint4(own.x, own.y, next.x, next.y), make_uint4(0, 0, 0, 0), bytes >> 2, (bytes & 3) * 8);
+    return make_uint2(r.x, r.y);
+}
+__device__ __forceinline__ uint32_t join_pieces(uint32_t own, uint32_t next, int bytes) {
+    return __funnelshift_r(own, next, bytes * 8);
+}
+template <typename E, typename V>
+__device__ __forceinline__ void store_shifted(E* row, int cols, int c, const V& own, const V& next) {
+    constexpr int B = sizeof(V), P = B / sizeof(E);
+    const int off = (int)(reinterpret_cast<uintptr_t>(row) % B);
+    const int lead = off ? (B - off) / (int)sizeof(E) : 0;      // elements before the first aligned piece
+    if (c == 0 && lead) {
+        const E* e = reinterpret_cast<const E*>(&own);
+#pragma unroll
+        for (int j = 0; j < P; ++j)
+            if (j < lead && j < cols) row[j] = e[j];
+    }
+    const int first = c + lead;
+    if (first >= cols) return;
+    const V out = lead ? join_pieces(own, next, lead * (int)sizeof(E)) : own;
+    if (first + P <= cols) {
+        *reinterpret_cast<V*>(row + first) = out;
+    } else {
+        const E* e = reinterpret_cast<const E*>(&out);
+#pragma unroll
+        for (int j = 0; j < P; ++j)
+            if (first + j < cols) row[first + j] = e[j];
+    }
+}
+__device__ __forceinline__ uint4 shuffle_down(const uint4& v) {
+    return make_uint4(__shfl_down_sync(~0u, v.x, 1), __shfl_down_sync(~0u, v.y, 1), __shfl_down_sync(~0u, v.z, 1),
+                      __shfl_down_sync(~0u, v.w, 1));
+}
+__device__ __forceinline__ uint2 shuffle_down(const uint2& v) {
+    return make_uint2(__shfl_down_sync(~0u, v.x, 1), __shfl_down_sync(~0u, v.y, 1));
+}
+__device__ __forceinline__ uint32_t shuffle_down(uint32_t v) { return __shfl_down_sync(~0u, v, 1); }
+// The next thread's piece: from the next lane, and for the last one what the next warp's
+// first lane left in shared memory.
+template <typename V>
+__device__ __forceinline__ V next_piece(const V& own, const V* edge, bool last_lane) {
+    V n = shuffle_down(own);
+    if (last_lane) n = *edge;
+    return n;
+}
+
+template <int P> struct BytePiece;
+template <> struct BytePiece<8> { using type = uint2; };
+template <> struct BytePiece<4> { using type = uint32_t; };
+
 // The row stays in registers: N pieces per thread, piece i of thread t at column
 // (i * threads + t) * kPiece. A group of 128 columns is 16 (or 32) neighbouring lanes.
-template <typename T, typename W, int N, bool QUANT>
+// !ALIGNED: rows of any alignment and length, read and written as aligned pieces that are
+// shifted into place. That takes twice the instructions, which then bound it (4000 x 8191 bf16
+// with a residual and an 8-bit output: 87 us, 2.7 TB/s; element by element 114 us).
+template <typename T, typename W, int N, bool QUANT, bool ALIGNED, bool STREAM>
 __global__ void __launch_bounds__(1024)
 rms_norm_kernel(RmsNormArgs a) {
     constexpr int P = kPiece<T>;
+    using Q = typename BytePiece<P>::type;
     __shared__ float part[32];
+    __shared__ uint4 edge_h[ALIGNED ? 1 : N * 32 + 1];
+    __shared__ uint4 edge_y[ALIGNED ? 1 : N * 32 + 1];
     const int64_t row = blockIdx.x;
     const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
     const T* res = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride : nullptr;
     const W* w = static_cast<const W*>(a.weight);
     T* h_out = a.h_out ? static_cast<T*>(a.h_out) + row * a.h_stride : nullptr;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int threads = blockDim.x, cols = (int)a.cols;
+    const int threads = blockDim.x, warps = threads >> 5, cols = (int)a.cols;
     uint4 qx[N], qr[N];
     float v[N][P];
+    if (ALIGNED) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int c = (i * threads + (int)threadIdx.x) * P;
-        qx[i] = qr[i] = make_uint4(0, 0, 0, 0);
-        if (c < cols) {
-            qx[i] = *reinterpret_cast<const uint4*>(x + c);
-            if (res) qr[i] = *reinterpret_cast<const uint4*>(res + c);
+        for (int i = 0; i < N; ++i) {
+            const int c = (i * threads + (int)threadIdx.x) * P;
+            qx[i] = qr[i] = make_uint4(0, 0, 0, 0);
+            if (c < cols) {
+                qx[i] = load_piece<STREAM>(x + c);
+                if (res) qr[i] = load_piece<STREAM>(res + c);
+            }
+        }
+    } else {
+        const RowLoader<T> lx(x, (uint32_t)cols, 0), lr(res, (uint32_t)cols, 0);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int u = i * threads + (int)threadIdx.x;
+            qx[i] = qr[i] = make_uint4(0, 0, 0, 0);
+            if (u * P < cols) {
+                qx[i] = lx(u);
+                if (res) qr[i] = lr(u);
+            }
         }
     }
     float sum = 0.0f;
@@ -159,21 +251,39 @@ rms_norm_kernel(RmsNormArgs a) {
         }
 #pragma unroll
         for (int j = 0; j < P; ++j) sum = fmaf(v[i][j], v[i][j], sum);
+        if (!ALIGNED && h_out && lane == 0) edge_h[i * warps + warp] = pack<T>(v[i]);
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
     if (lane == 0) part[warp] = sum;
     __syncthreads();
-    sum = lane < (threads >> 5) ? part[lane] : 0.0f;
+    sum = lane < warps ? part[lane] : 0.0f;
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
     const float r = rsqrtf(sum / (float)cols + a.eps);
+    uint4 out[N];               // the pieces of y
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int c = (i * threads + (int)threadIdx.x) * P;
-        if (c < cols) {
-            if (h_out) *reinterpret_cast<uint4*>(h_out + c) = pack<T>(v[i]);
-            float wv[P];
+        if (ALIGNED) {
+            if (h_out && c < cols) store_piece<STREAM>(h_out + c, pack<T>(v[i]));
+        } else if (h_out) {
+            const uint4 own = pack<T>(v[i]);
+            const uint4 next = next_piece(own, edge_h + i * warps + warp + 1, lane == 31);
+            if (c < cols) store_shifted<T, uint4>(h_out, cols, c, own, next);
+        }
+        float wv[P];
+        if (!ALIGNED) {
+            const RowLoader<W> lw(w, (uint32_t)cols, 0);
+            constexpr int PW = kPiece<W>;
+#pragma unroll
+            for (int j = 0; j < P; j += PW) {
+                float f[PW];
+                unpack<W>(c + j < cols ? lw((uint32_t)(c + j) / PW) : make_uint4(0, 0, 0, 0), f);
+#pragma unroll
+                for (int t = 0; t < PW; ++t) wv[j + t] = f[t];
+            }
+        } else if (c < cols) {
             if (sizeof(W) == sizeof(T)) {
                 unpack<T>(__ldg(reinterpret_cast<const uint4*>(w + c)), wv);
             } else {
@@ -183,74 +293,101 @@ rms_norm_kernel(RmsNormArgs a) {
                     wv[j] = f.x; wv[j + 1] = f.y; wv[j + 2] = f.z; wv[j + 3] = f.w;
                 }
             }
+        }
+        if (c < cols) {
 #pragma unroll
             for (int j = 0; j < P; ++j) v[i][j] = v[i][j] * r * wv[j];
         }
         if (!QUANT) {
-            if (c < cols) *reinterpret_cast<uint4*>(static_cast<T*>(a.y) + row * a.y_stride + c) = pack<T>(v[i]);
-            continue;
-        }
-        float m = kTiny;                    // columns past the end count as 0
-        if (c < cols) {
+            out[i] = pack<T>(v[i]);
+            if (ALIGNED && c < cols) store_piece<STREAM>(static_cast<T*>(a.y) + row * a.y_stride + c, out[i]);
+        } else {
+            float m = kTiny;                // columns past the end count as 0
+            if (c < cols) {
 #pragma unroll
-            for (int j = 0; j < P; ++j) m = max_nan(m, fabsf(v[i][j]));
-        }
+                for (int j = 0; j < P; ++j) m = max_nan(m, fabsf(v[i][j]));
+            }
 #pragma unroll
-        for (int o = kGroup / P / 2; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(~0u, m, o));
-        if (c >= cols) continue;
-        if (c % kGroup == 0) a.scales[row * a.scales_stride + c / kGroup] = m / kE4m3Max;
-        // the quotient by the scale as a product: one division per thread and not per value,
-        // within an ulp of 32 bits of it
-        const float inv = kE4m3Max / m;
-        uint8_t* y = static_cast<uint8_t*>(a.y) + row * a.y_stride + c;
-        uint32_t out[P / 4];
+            for (int o = kGroup / P / 2; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(~0u, m, o));
+            if (c < cols && c % kGroup == 0) a.scales[row * a.scales_stride + c / kGroup] = m / kE4m3Max;
+            // the quotient by the scale as a product: one division per thread and not per value,
+            // within an ulp of 32 bits of it
+            const float inv = kE4m3Max / m;
+            uint32_t b[2] = {0, 0};
 #pragma unroll
-        for (int j = 0; j < P; j += 4) {
-            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[i][j] * inv, v[i][j + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[i][j + 2] * inv, v[i][j + 3] * inv), __NV_SATFINITE, __NV_E4M3);
-            out[j / 4] = lo | hi << 16;
+            for (int j = 0; j < P; j += 4) {
+                const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[i][j] * inv, v[i][j + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+                const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[i][j + 2] * inv, v[i][j + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+                b[j / 4] = lo | hi << 16;
+            }
+            out[i] = make_uint4(b[0], b[1], 0, 0);
+            if (ALIGNED && c < cols) {
+                uint8_t* y = static_cast<uint8_t*>(a.y) + row * a.y_stride + c;
+                if (P == 8) store_piece<STREAM>(y, make_uint2(b[0], b[1]));
+                else store_piece<STREAM>(y, b[0]);
+            }
         }
-        if (P == 8) *reinterpret_cast<uint2*>(y) = make_uint2(out[0], out[P / 4 - 1]);
-        else *reinterpret_cast<uint32_t*>(y) = out[0];
+        if (!ALIGNED && lane == 0) edge_y[i * warps + warp] = out[i];
+    }
+    if (ALIGNED) return;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int c = (i * threads + (int)threadIdx.x) * P;
+        const uint4* edge = edge_y + i * warps + warp + 1;
+        if (QUANT) {
+            const Q own = *reinterpret_cast<const Q*>(&out[i]);
+            const Q next = next_piece(own, reinterpret_cast<const Q*>(edge), lane == 31);
+            if (c < cols) store_shifted<uint8_t, Q>(static_cast<uint8_t*>(a.y) + row * a.y_stride, cols, c, own, next);
+        } else {
+            const uint4 next = next_piece(out[i], edge, lane == 31);
+            if (c < cols) store_shifted<T, uint4>(static_cast<T*>(a.y) + row * a.y_stride, cols, c, out[i], next);
+        }
     }
 }
 
-// Pieces per thread and threads: few rows get many threads with a piece each (the time is
-// that of one row), many rows get up to 4 pieces per thread.
-template <typename T, typename W, bool QUANT>
+template <typename T, typename W, int N, bool QUANT, bool ALIGNED>
+void launch_n(const RmsNormArgs& a, int64_t pieces, cudaStream_t s) {
+    const int threads = (int)std::max<int64_t>(32, ((pieces + N - 1) / N + 31) / 32 * 32);
+    // With a residual, four arrays go through the L2 cache; beyond half of its 126 MB they only
+    // push each other out, and passing them through is faster (16384 x 8192 bf16, 8-bit output:
+    // 141 us against 173; 8192 x 4096: 37.9 against 40.9). Without one it is not (40000 x 2048
+    // bf16: 53.3 against 50.4).
+    const int64_t bytes = a.rows * a.cols * (int64_t)sizeof(T) * 3;
+    if (ALIGNED && a.residual && bytes > (int64_t(64) << 20)) rms_norm_kernel<T, W, N, QUANT, ALIGNED, ALIGNED><<<(unsigned)a.rows, threads, 0, s>>>(a);
+    else rms_norm_kernel<T, W, N, QUANT, ALIGNED, false><<<(unsigned)a.rows, threads, 0, s>>>(a);
+}
+
+// Pieces per thread: one for rows that all run at once (100 x 4096 bf16: 2.6 us, with two 3.0,
+// with four 3.9), two for more rows (16384 x 8192: 141 us, one 182, four 142), four for rows
+// that two do not hold.
+template <typename T, typename W, bool QUANT, bool ALIGNED>
 bool launch_pieces(const RmsNormArgs& a, cudaStream_t s) {
     const int64_t pieces = (a.cols + kPiece<T> - 1) / kPiece<T>;
-    int n = a.rows <= 296 ? 1 : 4;
-    while (n > 1 && pieces <= 128 * (n / 2)) n /= 2;
-    while (n < 4 && pieces > 1024 * n) n *= 2;
-    if (pieces > 1024 * n) return false;
-    const int threads = (int)std::max<int64_t>(32, ((pieces + n - 1) / n + 31) / 32 * 32);
-    const unsigned grid = (unsigned)a.rows;
-    if (n == 1) rms_norm_kernel<T, W, 1, QUANT><<<grid, threads, 0, s>>>(a);
-    else if (n == 2) rms_norm_kernel<T, W, 2, QUANT><<<grid, threads, 0, s>>>(a);
-    else rms_norm_kernel<T, W, 4, QUANT><<<grid, threads, 0, s>>>(a);
+    if (pieces > 4 * 1024) return false;
+    if (pieces > 2 * 1024) launch_n<T, W, 4, QUANT, ALIGNED>(a, pieces, s);
+    else if (pieces > 1024 || (a.rows > 296 && pieces > 32)) launch_n<T, W, 2, QUANT, ALIGNED>(a, pieces, s);
+    else launch_n<T, W, 1, QUANT, ALIGNED>(a, pieces, s);
     return true;
 }
 
-template <typename T, typename W>
+template <typename T, typename W, bool QUANT>
 void launch_typed(const RmsNormArgs& a, cudaStream_t s) {
-    // 16-byte pieces need their alignment everywhere, and rows that end with one; other rows
-    // and those too long for the registers go element by element.
     auto whole = [&](const void* p, int64_t stride, int64_t bytes, int64_t piece) {
         return !p || (reinterpret_cast<uintptr_t>(p) % piece == 0 && (a.rows <= 1 || stride * bytes % piece == 0));
     };
     const int64_t e = sizeof(T);
-    const bool pieces = a.cols % kPiece<T> == 0 && whole(a.x, a.x_stride, e, 16) && whole(a.residual, a.residual_stride, e, 16) &&
-                        whole(a.h_out, a.h_stride, e, 16) && reinterpret_cast<uintptr_t>(a.weight) % 16 == 0 &&
-                        (a.quantize ? whole(a.y, a.y_stride, 1, kPiece<T>) : whole(a.y, a.y_stride, e, 16));
-    if (pieces && (a.quantize ? launch_pieces<T, W, true>(a, s) : launch_pieces<T, W, false>(a, s))) return;
-    rms_norm_rows_kernel<T, W><<<(unsigned)a.rows, 256, 0, s>>>(a);
+    const bool aligned = a.cols % kPiece<T> == 0 && whole(a.x, a.x_stride, e, 16) && whole(a.residual, a.residual_stride, e, 16) &&
+                         whole(a.h_out, a.h_stride, e, 16) && reinterpret_cast<uintptr_t>(a.weight) % 16 == 0 &&
+                         (QUANT ? whole(a.y, a.y_stride, 1, kPiece<T>) : whole(a.y, a.y_stride, e, 16));
+    if (aligned ? launch_pieces<T, W, QUANT, true>(a, s) : launch_pieces<T, W, QUANT, false>(a, s)) return;
+    rms_norm_rows_kernel<T, W><<<(unsigned)a.rows, 256, 0, s>>>(a);      // rows too long for the registers
 }
 
 template <typename T>
 void launch_weights(const RmsNormArgs& a, cudaStream_t s) {
-    if (a.weight_dtype == ENGINE_F32) launch_typed<T, float>(a, s);
-    else launch_typed<T, T>(a, s);
+    if (a.weight_dtype == ENGINE_F32) a.quantize ? launch_typed<T, float, true>(a, s) : launch_typed<T, float, false>(a, s);
+    else a.quantize ? launch_typed<T, T, true>(a, s) : launch_typed<T, T, false>(a, s);
 }
 
 }  // namespace
@@ -258,7 +395,7 @@ void launch_weights(const RmsNormArgs& a, cudaStream_t s) {
 void launch_rms_norm(const RmsNormArgs& a, cudaStream_t s) {
     if (a.rows == 0 || a.cols == 0) return;
     switch (a.dtype) {
-        case ENGINE_F32: launch_typed<float, float>(a, s); break;
+        case ENGINE_F32: launch_weights<float>(a, s); break;
         case ENGINE_F16: launch_weights<__half>(a, s); break;
         case ENGINE_BF16: launch_weights<__nv_bfloat16>(a, s); break;
         default: fail(ENGINE_ERR_INVALID_ARG, "rms_norm: dtype must be F32, F16 or BF16");

@@ -24,6 +24,7 @@
 
 #include "common.h"
 #include "device_common.cuh"
+#include "row_vec.cuh"
 
 namespace pb {
 
@@ -272,52 +273,6 @@ template <typename T> __device__ __forceinline__ float vec_max(const uint4& v) {
     return fmaxf(x[0], x[1]);
 }
 
-// Vectors of a row that may start anywhere: one aligned load, or two and a shift by the
-// row's offset within 16 bytes. Nothing outside the row is read.
-template <typename T>
-struct RowLoader {
-    const T* row;
-    uint32_t n;                 // elements
-    const uint4* base;          // the aligned vector that holds the row's first element
-    int words, bits;            // the row's offset in it
-    __device__ __forceinline__ RowLoader(const T* r, uint32_t len) : row(r), n(len) {
-        const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(r) & 15);
-        base = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(r) - off);
-        words = (int)(off >> 2);
-        bits = (int)(off & 3) * 8;
-    }
-    // vectors before this one are aligned and whole
-    __device__ __forceinline__ uint32_t easy() const { return (words | bits) == 0 ? n / kVec<T> : 0; }
-    __device__ __forceinline__ uint4 operator()(uint32_t v) const {
-        const uint32_t i = v * kVec<T>;
-        // the two vectors lie inside the row unless v is its first or its last
-        if (v > 0 && i + 2 * kVec<T> <= n) {
-            const uint4 lo = __ldg(base + v), hi = __ldg(base + v + 1);
-            uint32_t s[5];
-            switch (words) {
-                case 0: s[0] = lo.x; s[1] = lo.y; s[2] = lo.z; s[3] = lo.w; s[4] = hi.x; break;
-                case 1: s[0] = lo.y; s[1] = lo.z; s[2] = lo.w; s[3] = hi.x; s[4] = hi.y; break;
-                case 2: s[0] = lo.z; s[1] = lo.w; s[2] = hi.x; s[3] = hi.y; s[4] = hi.z; break;
-                default: s[0] = lo.w; s[1] = hi.x; s[2] = hi.y; s[3] = hi.z; s[4] = hi.w; break;
-            }
-            return make_uint4(__funnelshift_r(s[0], s[1], bits), __funnelshift_r(s[1], s[2], bits),
-                              __funnelshift_r(s[2], s[3], bits), __funnelshift_r(s[3], s[4], bits));
-        }
-        uint32_t w[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (sizeof(T) == 4) {
-                w[j] = i + j < n ? __float_as_uint((float)row[i + j]) : 0xFF800000u;
-            } else {
-                const uint16_t* h = reinterpret_cast<const uint16_t*>(row);
-                const uint32_t low = kIsHalf<T> ? 0xFC00u : 0xFF80u;     // -inf
-                w[j] = (i + 2 * j < n ? h[i + 2 * j] : low) | ((i + 2 * j + 1 < n ? h[i + 2 * j + 1] : low) << 16);
-            }
-        }
-        return make_uint4(w[0], w[1], w[2], w[3]);
-    }
-};
-
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -513,7 +468,7 @@ sample_cluster_kernel(SampleArgs a, int shift, int ctas) {
     const uint32_t i_own = v0 * VEC + tid * VEC;        // first element of this thread's first vector
 
     cluster_arrive();                   // answered below: before memory of another CTA is written, it has started
-    const RowLoader<T> load(lg, V);
+    const RowLoader<T> load(lg, V, vec_none<T>().x & (sizeof(T) == 4 ? ~0u : 0xFFFFu));
     float top;
     {
         uint4 m = vec_none<T>();
