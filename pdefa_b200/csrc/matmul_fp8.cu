@@ -17,6 +17,7 @@
 // tokens have one each; their products come from shared memory as one broadcast load
 // per four columns, and the sum is one packed fp32x2 multiply-add per two columns.
 #include <algorithm>
+#include <cstdlib>
 #include <cuda.h>
 #include <cuda_fp16.h>
 
@@ -140,7 +141,7 @@ __device__ __forceinline__ int build_table(const TcArgs& p, int* table) {
 
 // Tiles are numbered with the token tiles of an expert innermost, so that CTAs that run
 // together read the same weight rows.
-template <int BT>
+template <int BT, int TN>
 __device__ __forceinline__ Tile tile_of(const TcArgs& p, const int* table, int token_tiles, int64_t t) {
     Tile r;
     if (!p.offsets) {
@@ -148,7 +149,7 @@ __device__ __forceinline__ Tile tile_of(const TcArgs& p, const int* table, int t
         r.expert = 0;
         r.row0 = (int)(t - (int64_t)nt * p.m_tiles) * BT;
         r.rows = min(BT, p.m - r.row0);
-        r.n0 = nt * kTileN;
+        r.n0 = nt * TN;
         return r;
     }
     const int* before = table + 2 * p.experts;
@@ -165,7 +166,7 @@ __device__ __forceinline__ Tile tile_of(const TcArgs& p, const int* table, int t
     r.expert = lo;
     r.row0 = table[lo] + (int)(local - (int64_t)nt * mine) * BT;
     r.rows = min(BT, table[p.experts + lo] - r.row0);
-    r.n0 = nt * kTileN;
+    r.n0 = nt * TN;
     return r;
 }
 
@@ -245,7 +246,7 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
             RingPos rp;
             int64_t it = 0;
             for (int64_t t = t0; t < total && !failed; t += tstep) {
-                const Tile tl = tile_of<BT>(p, table, token_tiles, t);
+                const Tile tl = tile_of<BT, kTileN>(p, table, token_tiles, t);
                 for (int kb = kb0; kb < kb1; ++kb) {
                     const int st = rp.slot;
                     if (rp.wrapped && !mbar_wait_bounded(&empty[st], rp.phase ^ 1u, p.wait_limit)) {
@@ -293,7 +294,7 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
         // scales: chunk c holds sa[token, kb] * sb[kb] for kScaleChunk k-blocks, [kb][token]
         RingPos cp;
         for (int64_t t = t0; t < total && !failed; t += tstep) {
-            const Tile tl = tile_of<BT>(p, table, token_tiles, t);
+            const Tile tl = tile_of<BT, kTileN>(p, table, token_tiles, t);
             const float* sa = p.sa + (int64_t)tl.row0 * p.lda_scales;
             const float* sb = p.sb + tl.expert * p.sb_expert + (tl.n0 / kTileN) * p.ldb_scales;
             for (int kc = kb0; kc < kb1 && !failed; kc += kScaleChunk) {
@@ -327,7 +328,7 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
         RingPos ap, cp;
         for (int64_t t = t0; t < total && !failed; t += tstep) {
-            mine = tile_of<BT>(p, table, token_tiles, t);
+            mine = tile_of<BT, kTileN>(p, table, token_tiles, t);
 #pragma unroll
             for (int i = 0; i < S::kCols; ++i) acc[i] = 0.0f;
             for (int kb = kb0; kb < kb1; ++kb) {
@@ -426,6 +427,373 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
     }
 }
 
+// ---------------------------------------------------------------------------
+// Many tokens: tiles of 128 * CG tokens (TMEM lanes, 128 per CTA) times 256 weight rows (TMEM
+// columns). CG = 2 is a pair of CTAs on one tile: each brings its own tokens and half of the
+// weight rows, and the tensor cores of both read both halves, so that a CTA moves 32 KB per
+// k-block instead of 48.
+// ---------------------------------------------------------------------------
+constexpr int kWideN = 256;
+constexpr int kWideEpi = 8;
+constexpr int kWideThreads = 128 + 32 * kWideEpi;
+constexpr int kWideCols = kWideN / 2;           // columns of an epilogue thread: one weight block
+constexpr uint32_t kWideScales = kScaleChunk * (128 + 2) * 4;
+
+__device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void wide_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+    if (CG == 1)
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void wide_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+    if (CG == 1)
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
+// Arrival on the barrier at this address in every CTA of the group once the products
+// issued so far have completed.
+template <int CG>
+__device__ __forceinline__ void wide_commit(uint64_t* bar) {
+    if (CG == 1) umma_commit(bar);
+    else
+        asm volatile("{\n\t.reg .b16 m;\n\tmov.b16 m, 3;\n\t"
+                     "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n\t}"
+                     ::"r"(smem_u32(bar)) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void wide_mma(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc) {
+    if (CG == 1)
+        asm volatile(
+            "{\n\t.reg .pred pf, pt;\n\t.reg .b64 a1, b1, a2, b2, a3, b3;\n\t"
+            "setp.ne.u32 pf, 0, 0;\n\tsetp.eq.u32 pt, 0, 0;\n\t"
+            "add.s64 a1, %1, 2;\n\tadd.s64 b1, %2, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 b2, %2, 4;\n\t"
+            "add.s64 a3, %1, 6;\n\tadd.s64 b3, %2, 6;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, pf;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a1, b1, %3, pt;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a2, b2, %3, pt;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a3, b3, %3, pt;\n\t}"
+            ::"r"(d), "l"(da), "l"(db), "r"(idesc) : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred pf, pt;\n\t.reg .b64 a1, b1, a2, b2, a3, b3;\n\t"
+            "setp.ne.u32 pf, 0, 0;\n\tsetp.eq.u32 pt, 0, 0;\n\t"
+            "add.s64 a1, %1, 2;\n\tadd.s64 b1, %2, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 b2, %2, 4;\n\t"
+            "add.s64 a3, %1, 6;\n\tadd.s64 b3, %2, 6;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, pf;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a1, b1, %3, pt;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a2, b2, %3, pt;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a3, b3, %3, pt;\n\t}"
+            ::"r"(d), "l"(da), "l"(db), "r"(idesc) : "memory");
+}
+
+// 32 consecutive fp32 columns of this thread's TMEM lane; no wait.
+__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+
+// Registers: the launch gives every thread kWideRegs; the four warps of loads, products and
+// scales hand most of theirs to the eight epilogue warps, whose 128 sums and 64 values in
+// flight would not fit otherwise. The two sums are equal, as the instruction needs.
+constexpr int kWideRegs = 168, kWideRegsLess = 72, kWideRegsMore = 216;
+static_assert(128 * kWideRegsLess + 32 * kWideEpi * kWideRegsMore <= kWideThreads * kWideRegs, "register split");
+
+__device__ __forceinline__ uint32_t pack2(float a, float b, int dtype) {
+    if (dtype == ENGINE_F16) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Roles and bounded waits as above. Pairs: CTA 0 of the cluster issues the products for both;
+// both CTAs' loads complete on its `full` barriers, its commits arrive in both CTAs, and both
+// epilogues hand accumulators back to it.
+template <int CG>
+__global__ void __launch_bounds__(kWideThreads, 1)
+matmul_fp8_wide_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmA, const TcArgs p) {
+    constexpr int BT = 128 * CG;                             // tokens of a tile
+    constexpr uint32_t kA = 128 * kBlock, kB = kWideN / CG * kBlock;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    uint8_t* const smem = smem_raw + (base - raw);
+    const int stages = p.stages;
+    // [token slots | weight slots | scales | barriers | table], slots 1024-aligned
+    const uint32_t ring_b = base + (uint32_t)stages * kA;
+    float* const scales = reinterpret_cast<float*>(smem + (size_t)stages * (kA + kB));
+    uint64_t* const full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(scales) + 2 * kWideScales);
+    uint64_t* const empty = full + stages;
+    uint64_t* const tfull = empty + stages;
+    uint64_t* const tempty = tfull + 2;
+    uint64_t* const sfull = tempty + 2;
+    uint64_t* const sempty = sfull + 2;
+    uint64_t* const mma_done = sempty + 2;
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
+    int* const tile_count = reinterpret_cast<int*>(tmem_slot + 1);
+    int* const table = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(full) + kBarrierBytes);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = CG == 2 ? cluster_rank() : 0;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < stages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&tfull[i], 1); mbar_init(&tempty[i], kWideEpi * CG); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&sfull[i], 1); mbar_init(&sempty[i], kWideEpi); }
+        mbar_init(mma_done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        if (CG == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        }
+    }
+    if (warp == 2) {
+        const int n = p.offsets ? build_table<BT>(p, table) : p.m_tiles;
+        if (lane == 0) *tile_count = n;
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (CG == 2) cluster_sync();                             // the other CTA's barriers and TMEM are ready too
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+    const int token_tiles = *tile_count;
+    const int64_t total = (int64_t)token_tiles * p.n_tiles;
+    const int64_t t0 = blockIdx.x / CG, tstep = gridDim.x / CG;
+    bool failed = false;
+
+    if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideRegsLess));
+    if (warp == 0) {
+        if (lane == 0) {
+            RingPos rp;
+            int64_t it = 0;
+            for (int64_t t = t0; t < total && !failed; t += tstep) {
+                const Tile tl = tile_of<BT, kWideN>(p, table, token_tiles, t);
+                for (int kb = 0; kb < p.nkb; ++kb) {
+                    const int st = rp.slot;
+                    if (rp.wrapped && !mbar_wait_bounded(&empty[st], rp.phase ^ 1u, p.wait_limit)) {
+                        atomicExch(p.err, 31);
+                        failed = true;
+                        break;
+                    }
+                    rp.next(stages);
+                    ++it;
+                    if (rank == 0) mbar_expect_tx(&full[st], CG * (kA + kB));
+                    const uint32_t bar = CG == 2 ? mapa(smem_u32(&full[st]), 0) : smem_u32(&full[st]);
+                    wide_load_2d<CG>(base + (uint32_t)st * kA, &tmA, bar, kb * kBlock, tl.row0 + (int)rank * 128);
+                    // 128 weight rows per box
+                    for (int h = 0; h < 2 / CG; ++h)
+                        wide_load_3d<CG>(ring_b + (uint32_t)st * kB + h * (128 * kBlock), &tmB, bar, kb * kBlock,
+                                         tl.n0 + ((int)rank + h) * 128, tl.expert);
+                }
+            }
+            // the last load of every slot has landed before the CTA (or its pair) may exit
+            if (rank == 0)
+                for (int64_t k = it > stages ? it - stages : 0; k < it; ++k)
+                    if (!mbar_wait_bounded(&full[k % stages], (uint32_t)((k / stages) & 1))) atomicExch(p.err, 32);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            const uint32_t idesc = (1u << 4) | ((uint32_t)(kWideN >> 3) << 17) | ((uint32_t)(BT >> 4) << 24);
+            RingPos rp, ap;
+            for (int64_t t = t0; t < total && !failed; t += tstep) {
+                for (int kb = 0; kb < p.nkb; ++kb) {
+                    const int st = rp.slot, buf = ap.slot;
+                    if ((ap.wrapped && !mbar_wait_bounded(&tempty[buf], ap.phase ^ 1u, p.wait_limit)) ||
+                        !mbar_wait_bounded(&full[st], rp.phase, p.wait_limit)) {
+                        atomicExch(p.err, 33);
+                        failed = true;
+                        break;
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    wide_mma<CG>(tmem + (uint32_t)(buf * kWideN), make_smem_desc(base + (uint32_t)st * kA, 128),
+                                 make_smem_desc(ring_b + (uint32_t)st * kB, 128), idesc);
+                    wide_commit<CG>(&empty[st]);
+                    wide_commit<CG>(&tfull[buf]);
+                    rp.next(stages);
+                    ap.next(2);
+                }
+            }
+            wide_commit<CG>(mma_done);
+        }
+        __syncwarp();
+    } else if (warp == 2) {
+        // scales: chunk c holds sa[token] for kScaleChunk k-blocks, then sb of the two weight blocks
+        RingPos cp;
+        for (int64_t t = t0; t < total && !failed; t += tstep) {
+            const Tile tl = tile_of<BT, kWideN>(p, table, token_tiles, t);
+            const int rows = tl.rows - (int)rank * 128;
+            const float* sa = p.sa + (int64_t)(tl.row0 + (int)rank * 128) * p.lda_scales;
+            const float* sb = p.sb + tl.expert * p.sb_expert + (tl.n0 / kBlock) * p.ldb_scales;
+            const bool second = tl.n0 + kBlock < p.n;
+            for (int kc = 0; kc < p.nkb && !failed; kc += kScaleChunk) {
+                if (cp.wrapped && !warp_wait(&sempty[cp.slot], cp.phase ^ 1u, p.wait_limit)) {
+                    if (lane == 0) atomicExch(p.err, 34);
+                    failed = true;
+                    break;
+                }
+                float* dst = scales + cp.slot * (kWideScales / 4);
+                float v[4][kScaleChunk];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < kScaleChunk; ++j)
+                        v[i][j] = i * 32 + lane < rows && kc + j < p.nkb ? __ldg(sa + (int64_t)(i * 32 + lane) * p.lda_scales + kc + j) : 0.0f;
+                if (lane < 2 * kScaleChunk) {
+                    const int blk = lane / kScaleChunk, j = lane % kScaleChunk;
+                    dst[kScaleChunk * 128 + lane] = (blk == 0 || second) && kc + j < p.nkb ? __ldg(sb + blk * p.ldb_scales + kc + j) : 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < kScaleChunk; ++j) dst[j * 128 + i * 32 + lane] = v[i][j];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sfull[cp.slot]);
+                cp.next(2);
+            }
+        }
+        __syncwarp();
+    }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWideRegsMore));
+        const int q = warp & 3, half = (warp - 4) >> 2;      // TMEM lane quarter, weight block
+        const uint32_t lanes = (uint32_t)(q * 32) << 16;
+        const int tok = q * 32 + lane;
+        float acc[kWideCols];
+        RingPos ap, cp;
+        for (int64_t t = t0; t < total && !failed; t += tstep) {
+            const Tile tl = tile_of<BT, kWideN>(p, table, token_tiles, t);
+#pragma unroll
+            for (int i = 0; i < kWideCols; ++i) acc[i] = 0.0f;
+            for (int kb = 0; kb < p.nkb; ++kb) {
+                const int in_chunk = kb % kScaleChunk;
+                if ((in_chunk == 0 && !warp_wait(&sfull[cp.slot], cp.phase, p.wait_limit)) ||
+                    !warp_wait(&tfull[ap.slot], ap.phase, p.wait_limit)) {
+                    if (lane == 0) atomicExch(p.err, 35);
+                    failed = true;
+                    break;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t src = tmem + lanes + (uint32_t)(ap.slot * kWideN + half * kWideCols);
+                const float* sc = scales + cp.slot * (kWideScales / 4);
+                uint32_t r[2][32];
+                tmem_ld32_async(src, r[0]);
+                const float s1 = sc[in_chunk * 128 + tok] * sc[kScaleChunk * 128 + half * kScaleChunk + in_chunk];
+                const float2 s2 = make_float2(s1, s1);
+#pragma unroll
+                for (int c = 0; c < kWideCols / 32; ++c) {
+                    tmem_wait_ld();
+                    if (c + 1 < kWideCols / 32) tmem_ld32_async(src + (c + 1) * 32, r[(c + 1) & 1]);
+                    else {
+                        // everything is in registers: the tensor core may refill the buffer
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (CG == 1) mbar_arrive(&tempty[ap.slot]);
+                            else mbar_arrive_cluster(mapa(smem_u32(&tempty[ap.slot]), 0));
+                        }
+                    }
+                    const uint32_t(&v)[32] = r[c & 1];
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        float* d = acc + c * 32 + j;
+                        const float2 o = __ffma2_rn(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), s2, make_float2(d[0], d[1]));
+                        d[0] = o.x;
+                        d[1] = o.y;
+                    }
+                }
+                ap.next(2);
+                if (in_chunk == kScaleChunk - 1 || kb == p.nkb - 1) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sempty[cp.slot]);
+                    cp.next(2);
+                }
+            }
+            if (failed) continue;
+            const int m = tok + (int)rank * 128, n0 = tl.n0 + half * kWideCols;
+            if (m < tl.rows) {
+                const int64_t at = (int64_t)(tl.row0 + m) * p.ldo + n0;
+                if (p.out_dtype == ENGINE_F32) {
+                    float* o = static_cast<float*>(p.out) + at;
+#pragma unroll
+                    for (int i = 0; i < kWideCols; i += 4)
+                        if (n0 + i + 4 <= p.n) *reinterpret_cast<float4*>(o + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+                        else
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                if (n0 + i + j < p.n) o[i + j] = acc[i + j];
+                } else {
+                    uint16_t* o = static_cast<uint16_t*>(p.out) + at;
+#pragma unroll
+                    for (int i = 0; i < kWideCols; i += 8)
+                        if (n0 + i + 8 <= p.n)
+                            *reinterpret_cast<uint4*>(o + i) =
+                                make_uint4(pack2(acc[i], acc[i + 1], p.out_dtype), pack2(acc[i + 2], acc[i + 3], p.out_dtype),
+                                           pack2(acc[i + 4], acc[i + 5], p.out_dtype), pack2(acc[i + 6], acc[i + 7], p.out_dtype));
+                        else
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                if (n0 + i + j < p.n) store_out(p.out, p.out_dtype, at + i + j, acc[i + j]);
+                }
+            }
+        }
+        if (p.offsets) {
+            // rows before the first and after the last expert's
+            const int lo = table[0], hi = table[2 * p.experts - 1];
+            const int tid = threadIdx.x - 128;
+            for (int64_t i = (int64_t)blockIdx.x; i < (int64_t)lo + (p.m - hi); i += gridDim.x) {
+                const int64_t row = i < lo ? i : hi + (i - lo);
+                for (int n = tid; n < p.n; n += 32 * kWideEpi) store_out(p.out, p.out_dtype, row * p.ldo + n, 0.0f);
+            }
+        }
+    }
+
+    // TMEM is freed, and a pair left, once every issued product has completed.
+    __syncthreads();
+    if (warp == 1) {
+        if (!mbar_wait_bounded(mma_done, 0) && lane == 0) atomicExch(p.err, 36);
+        __syncwarp();
+    }
+    if (CG == 2) {
+        __syncwarp();
+        cluster_sync();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
 // Rows of bytes into rows of `ld` bytes (a multiple of 16), for operands that TMA cannot read.
 __global__ void __launch_bounds__(256)
 repack_rows_kernel(const uint8_t* src, int64_t ld_src, int64_t group_src, uint8_t* dst, int64_t ld, int64_t rows, int64_t cols,
@@ -469,6 +837,35 @@ void launch_tc(const TcArgs& args, int64_t grid, const CUtensorMap& tmB, const C
     cfg.attrs = at;
     cfg.numAttrs = SPLIT ? 1 : 0;
     PB_CUDA(cudaLaunchKernelEx(&cfg, matmul_fp8_kernel<BT, SPLIT>, tmB, tmA, p));
+}
+
+template <int CG>
+void launch_wide(const TcArgs& args, int64_t tiles, int sms, const CUtensorMap& tmB, const CUtensorMap& tmA, int device, cudaStream_t s) {
+    TcArgs p = args;
+    constexpr uint32_t stage = 128 * kBlock + kWideN / CG * kBlock;
+    const uint32_t fixed = 1024 + 2 * kWideScales + kBarrierBytes + p.table_bytes;
+    p.stages = (int)std::min<uint32_t>(8, (227u * 1024u - fixed) / stage);
+    static bool ready[64] = {};
+    if (device >= 64 || !ready[device]) {
+        // a build with fewer registers per thread would leave the epilogue waiting for ones that are not there
+        cudaFuncAttributes attr;
+        PB_CUDA(cudaFuncGetAttributes(&attr, matmul_fp8_wide_kernel<CG>));
+        if (attr.numRegs != kWideRegs) fail(ENGINE_ERR_RUNTIME, "matmul_fp8: built with an unexpected number of registers");
+        PB_CUDA(cudaFuncSetAttribute(matmul_fp8_wide_kernel<CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+        if (device < 64) ready[device] = true;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(tiles, sms / CG) * CG));
+    cfg.blockDim = dim3(kWideThreads);
+    cfg.dynamicSmemBytes = fixed + (size_t)p.stages * stage;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = CG;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    PB_CUDA(cudaLaunchKernelEx(&cfg, matmul_fp8_wide_kernel<CG>, tmB, tmA, p));
 }
 
 }  // namespace
@@ -534,8 +931,10 @@ void launch_matmul_fp8(const MatmulFp8Args& g, cudaStream_t s) {
     // Tokens of a tile: the smallest width that holds the rows (an expert's average), so that
     // few tokens do not pay for a wide tile's empty columns.
     const int64_t rows = g.offsets ? (g.m + experts - 1) / experts : g.m;
-    const int bt = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
-    p.m_tiles = (int)((g.m + bt - 1) / bt);
+    const int wide = (getenv("WIDE") ? atoi(getenv("WIDE")) : 2) * (rows > 128 && reinterpret_cast<uintptr_t>(g.out) % 16 == 0 && g.ldo * (g.out_dtype == ENGINE_F32 ? 4 : 2) % 16 == 0);
+    const int bt = wide ? 128 : rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+    const int tokens = wide ? 128 * wide : bt;
+    p.m_tiles = (int)((g.m + tokens - 1) / tokens);
 
     CUtensorMap tmA, tmB;
     {
@@ -549,6 +948,13 @@ void launch_matmul_fp8(const MatmulFp8Args& g, cudaStream_t s) {
         if (!encode_box_map(&tmB, 1, 3, b, dims, st, box, true)) fail(ENGINE_ERR_INVALID_ARG, "matmul_fp8: tensor map of b refused");
     }
 
+    if (wide) {
+        p.n_tiles = (int)((g.n + kWideN - 1) / kWideN);
+        const int64_t tiles = (g.offsets ? std::min<int64_t>(g.m, experts + g.m / tokens) : p.m_tiles) * p.n_tiles;
+        if (wide == 1) launch_wide<1>(p, tiles, sms, tmB, tmA, device, s);
+        else launch_wide<2>(p, tiles, sms, tmB, tmA, device, s);
+        return;
+    }
     // Token tiles there can be at most: one per expert with rows, and one per full tile.
     const int64_t tiles = (g.offsets ? std::min<int64_t>(g.m, experts + g.m / bt) : p.m_tiles) * p.n_tiles;
     // Few tiles: a cluster of 2, 4 or 8 CTAs per tile, as long as each still gets two k-blocks
