@@ -350,13 +350,6 @@ __device__ __forceinline__ void store_chunk_staging(const TcParams& p, const flo
     }
 }
 
-__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int c0, int c1) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
-                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(c0), "r"(c1) : "memory");
-}
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_read0() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait0() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 // Named barriers 1 and 2 (one per epilogue group of 128 threads); the ids are
 // immediates so the kernel reserves only the barriers it uses.
 __device__ __forceinline__ void group_bar(int grp) {
@@ -888,7 +881,7 @@ bool pixel_dense(const TView& v) {
 }  // namespace
 
 bool encode_box_map(void* map, int elem_bytes, int rank, const void* ptr, const uint64_t* dims,
-                    const uint64_t* strides_bytes, const uint32_t* box, bool swizzle128) {
+                    const uint64_t* strides_bytes, const uint32_t* box, int swizzle) {
     if (rank < 1 || rank > 5 || (elem_bytes != 1 && elem_bytes != 4)) return false;
     load_driver_fns();
     cuuint64_t d[5], st[4];
@@ -898,7 +891,7 @@ bool encode_box_map(void* map, int elem_bytes, int rank, const void* ptr, const 
     return g_tiled(static_cast<CUtensorMap*>(map),
                    elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, (cuuint32_t)rank,
                    const_cast<void*>(ptr), d, st, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+                   swizzle ? swizzle_of(swizzle) : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 bool conv_tc_supported(const ConvArgs& a, int op_dt, const char** why) {

@@ -105,11 +105,11 @@ void launch_conv_direct(const ConvArgs& a, cudaStream_t s);
 // residual; threads gather im2col rows into shared memory. weight: as launch_conv_simt.
 // err: device error word for bounded waits.
 // TMA tensor map over uint8 (elem_bytes 1) or fp32 (4) data of `rank` dims (innermost
-// first; byte strides of dims 1..rank-1), no swizzle or rows of 128 swizzled bytes, zero
-// fill out of bounds; `map` is a 64-byte-aligned CUtensorMap. False when the driver
-// refuses the parameters.
+// first; byte strides of dims 1..rank-1), no swizzle (0) or swizzled rows of 64 or 128
+// bytes, zero fill out of bounds; `map` is a 64-byte-aligned CUtensorMap. False when the
+// driver refuses the parameters.
 bool encode_box_map(void* map, int elem_bytes, int rank, const void* ptr, const uint64_t* dims,
-                    const uint64_t* strides_bytes, const uint32_t* box, bool swizzle128 = false);
+                    const uint64_t* strides_bytes, const uint32_t* box, int swizzle = 0);
 bool conv_stem_tc_supported(const ConvArgs& a);
 void launch_conv_stem_tc(const ConvArgs& a, int* err, cudaStream_t s);
 

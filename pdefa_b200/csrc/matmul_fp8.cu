@@ -17,7 +17,6 @@
 // tokens have one each; their products come from shared memory as one broadcast load
 // per four columns, and the sum is one packed fp32x2 multiply-add per two columns.
 #include <algorithm>
-#include <cstdlib>
 #include <cuda.h>
 #include <cuda_fp16.h>
 
@@ -44,6 +43,7 @@ struct TcArgs {
     const float* sb; int64_t ldb_scales, sb_expert;
     void* out; int64_t ldo; int out_dtype;
     uint32_t table_bytes;               // the experts' tile table in shared memory (12 KB for the most experts)
+    int wide_out;                       // output rows start at multiples of 16 bytes
     int* err;
     long long wait_limit;
 };
@@ -69,10 +69,10 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, long l
     return __all_sync(~0u, mbar_wait_bounded(bar, parity, limit));
 }
 
-// One k-block: four K = 32 products into a fresh accumulator, then a commit to the
-// ring slot's and to the accumulator's barrier.
-__device__ __forceinline__ void mma_kblock(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint64_t* slot_free,
-                                           uint64_t* acc_full) {
+// One k-block: four K = 32 products into a fresh accumulator, then a commit to the ring
+// slot's barrier, which tells the loads that the slot is free and the epilogue that the
+// accumulator is full.
+__device__ __forceinline__ void mma_kblock(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint64_t* done) {
     asm volatile(
         "{\n\t.reg .pred pf, pt;\n\t.reg .b64 a1, b1, a2, b2, a3, b3;\n\t"
         "setp.ne.u32 pf, 0, 0;\n\tsetp.eq.u32 pt, 0, 0;\n\t"
@@ -82,9 +82,8 @@ __device__ __forceinline__ void mma_kblock(uint32_t d, uint64_t da, uint64_t db,
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a1, b1, %3, pt;\n\t"
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a2, b2, %3, pt;\n\t"
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a3, b3, %3, pt;\n\t"
-        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%4];\n\t"
-        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t}"
-        ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(smem_u32(slot_free)), "r"(smem_u32(acc_full))
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%4];\n\t}"
+        ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(smem_u32(done))
         : "memory");
 }
 
@@ -93,7 +92,7 @@ struct Shape {
     static constexpr int kEpi = BT >= 128 ? 8 : 4;                  // epilogue warps
     static constexpr int kThreads = 128 + 32 * kEpi;
     static constexpr int kCols = BT * 4 / kEpi;                     // columns of an epilogue thread
-    static constexpr int kBufs = BT == 256 ? 2 : 4;                 // TMEM accumulators
+    static constexpr int kBufs = 4;                                 // TMEM accumulators
     static constexpr int kTmemCols = kBufs * BT;                    // 64 .. 512
     static constexpr uint32_t kBBytes = BT * kBlock;
     static constexpr uint32_t kScaleBytes = kScaleChunk * BT * 4;   // of one of two chunks
@@ -176,7 +175,7 @@ __device__ __forceinline__ void store_out(void* out, int dtype, int64_t i, float
     else static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
 }
 
-// Roles: warp 0 brings operands (TMA), warp 1 issues the products and owns TMEM, warp 2
+// Roles: warps 0 and 3 bring operands (TMA), warp 1 issues the products and owns TMEM, warp 2
 // brings scales, warps 4 and up are the epilogue. Every wait is bounded; one that runs
 // out records a code in the device's error word and ends its role, after which the
 // others' waits run out too; loads and products in flight are waited for before exit.
@@ -195,9 +194,8 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
     const uint32_t ring_b = base + (uint32_t)stages * kABytes;
     float* const scales = reinterpret_cast<float*>(smem + (size_t)stages * (kABytes + S::kBBytes));
     uint64_t* const full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(scales) + 2 * S::kScaleBytes);
-    uint64_t* const empty = full + stages;
-    uint64_t* const tfull = empty + stages;
-    uint64_t* const tempty = tfull + S::kBufs;
+    uint64_t* const done = full + stages;
+    uint64_t* const tempty = done + stages;
     uint64_t* const sfull = tempty + S::kBufs;
     uint64_t* const sempty = sfull + 2;
     uint64_t* const mma_done = sempty + 2;
@@ -207,8 +205,8 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < stages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-        for (int i = 0; i < S::kBufs; ++i) { mbar_init(&tfull[i], 1); mbar_init(&tempty[i], S::kEpi); }
+        for (int i = 0; i < stages; ++i) { mbar_init(&full[i], 2); mbar_init(&done[i], 1); }
+        for (int i = 0; i < S::kBufs; ++i) mbar_init(&tempty[i], S::kEpi);
         for (int i = 0; i < 2; ++i) { mbar_init(&sfull[i], 1); mbar_init(&sempty[i], S::kEpi); }
         mbar_init(mma_done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -241,24 +239,27 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
     Tile mine{0, 0, 0, 0};
     bool failed = false;
 
-    if (warp == 0) {
+    if (warp == 0 || warp == 3) {
+        // Weights from one warp, tokens from another: issuing a load takes a thread some 150
+        // cycles, and both from one held up the narrow tiles.
         if (lane == 0) {
+            const bool weights = warp == 0;
             RingPos rp;
             int64_t it = 0;
             for (int64_t t = t0; t < total && !failed; t += tstep) {
                 const Tile tl = tile_of<BT, kTileN>(p, table, token_tiles, t);
                 for (int kb = kb0; kb < kb1; ++kb) {
                     const int st = rp.slot;
-                    if (rp.wrapped && !mbar_wait_bounded(&empty[st], rp.phase ^ 1u, p.wait_limit)) {
+                    if (rp.wrapped && !mbar_wait_bounded(&done[st], rp.phase ^ 1u, p.wait_limit)) {
                         atomicExch(p.err, 21);
                         failed = true;
                         break;
                     }
                     rp.next(stages);
                     ++it;
-                    mbar_expect_tx(&full[st], kABytes + S::kBBytes);
-                    tma_load_3d(base + (uint32_t)st * kABytes, &tmB, &full[st], kb * kBlock, tl.n0, tl.expert);
-                    tma_load_2d(ring_b + (uint32_t)st * S::kBBytes, &tmA, &full[st], kb * kBlock, tl.row0);
+                    mbar_expect_tx(&full[st], weights ? kABytes : S::kBBytes);
+                    if (weights) tma_load_3d(base + (uint32_t)st * kABytes, &tmB, &full[st], kb * kBlock, tl.n0, tl.expert);
+                    else tma_load_2d(ring_b + (uint32_t)st * S::kBBytes, &tmA, &full[st], kb * kBlock, tl.row0);
                 }
             }
             // the last load of every slot has landed before the CTA may exit
@@ -282,7 +283,7 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     mma_kblock(tmem + (uint32_t)(buf * BT), make_smem_desc(base + (uint32_t)st * kABytes, 128),
-                               make_smem_desc(ring_b + (uint32_t)st * S::kBBytes, 128), idesc, &empty[st], &tfull[buf]);
+                               make_smem_desc(ring_b + (uint32_t)st * S::kBBytes, 128), idesc, &done[st]);
                     rp.next(stages);
                     ap.next(S::kBufs);
                 }
@@ -326,7 +327,7 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
         const int q = warp & 3;                           // TMEM lane quarter
         const int c0 = ((warp - 4) >> 2) * S::kCols;      // first column of this warp's group
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
-        RingPos ap, cp;
+        RingPos rp, ap, cp;      // done, accumulators, scales
         for (int64_t t = t0; t < total && !failed; t += tstep) {
             mine = tile_of<BT, kTileN>(p, table, token_tiles, t);
 #pragma unroll
@@ -334,7 +335,7 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
             for (int kb = kb0; kb < kb1; ++kb) {
                 const int in_chunk = (kb - kb0) % kScaleChunk;
                 if ((in_chunk == 0 && !warp_wait(&sfull[cp.slot], cp.phase, p.wait_limit)) ||
-                    !warp_wait(&tfull[ap.slot], ap.phase, p.wait_limit)) {
+                    !warp_wait(&done[rp.slot], rp.phase, p.wait_limit)) {
                     if (lane == 0) atomicExch(p.err, 25);
                     failed = true;
                     break;
@@ -366,6 +367,7 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
                         d[0] = lo.x; d[1] = lo.y; d[2] = hi.x; d[3] = hi.y;
                     }
                 }
+                rp.next(stages);
                 ap.next(S::kBufs);
                 if (in_chunk == kScaleChunk - 1 || kb == kb1 - 1) {
                     __syncwarp();
@@ -436,7 +438,7 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
 constexpr int kWideN = 256;
 constexpr int kWideEpi = 8;
 constexpr int kWideThreads = 128 + 32 * kWideEpi;
-constexpr int kWideCols = kWideN / 2;           // columns of an epilogue thread: one weight block
+constexpr int kWideCols = kWideN * 4 / kWideEpi;    // columns of an epilogue thread
 constexpr uint32_t kWideScales = kScaleChunk * (128 + 2) * 4;
 
 __device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
@@ -520,13 +522,68 @@ __device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t (&r)[32
 constexpr int kWideRegs = 168, kWideRegsLess = 72, kWideRegsMore = 216;
 static_assert(128 * kWideRegsLess + 32 * kWideEpi * kWideRegsMore <= kWideThreads * kWideRegs, "register split");
 
-__device__ __forceinline__ uint32_t pack2(float a, float b, int dtype) {
-    if (dtype == ENGINE_F16) {
-        const __half2 h = __floats2half2_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
+// The warp's 32 rows (one per lane) of kWideCols sums to rows of the output, `rows` of which
+// are this tile's: through the warp's own shared memory in chunks of 128 bytes per row, whose
+// 16-byte pieces are swizzled against bank conflicts in the pattern of the output's tensor map.
+// Full tiles leave by TMA while the warp goes on; rows that are not aligned for it, or
+// belong to the next expert, are copied out by the warp. One fence and one pair of TMA
+// stores per 256 bytes of a row: issuing them takes a warp some 400 cycles (a tile of 8192 x
+// 8192 x 4096 has 32000).
+constexpr int kWideChunk = 32 * 128, kWideChunks = 2, kWideStage = kWideChunks * kWideChunk;
+template <typename T> __device__ __forceinline__ uint4 out_piece(const float* v);
+template <> __device__ __forceinline__ uint4 out_piece<float>(const float* v) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+}
+template <> __device__ __forceinline__ uint4 out_piece<__half>(const float* v) {
+    uint4 q;
+    __half2* h = reinterpret_cast<__half2*>(&q);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    return q;
+}
+template <> __device__ __forceinline__ uint4 out_piece<__nv_bfloat16>(const float* v) {
+    uint4 q;
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&q);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    return q;
+}
+template <typename T>
+__device__ __forceinline__ void wide_store(const TcArgs& p, const CUtensorMap* tmO, const float (&acc)[kWideCols], uint8_t* stage,
+                                           int row0, int rows, int n0) {
+    constexpr int kPer = 128 / sizeof(T), kPiece = 16 / sizeof(T);   // values of a chunk's row and of a piece
+    const int lane = threadIdx.x & 31;
+    const bool tma = p.wide_out && rows >= 32;
+#pragma unroll
+    for (int c = 0; c < kWideCols; c += kWideChunks * kPer) {
+        if (lane == 0) bulk_wait_read<0>();                          // what was here has left
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < kWideChunks * 8; ++j)
+            *reinterpret_cast<uint4*>(stage + j / 8 * kWideChunk + lane * 128 + ((j ^ lane) & 7) * 16) = out_piece<T>(acc + c + j * kPiece);
+        if (tma) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+#pragma unroll
+                for (int h = 0; h < kWideChunks; ++h)
+                    if (n0 + c + h * kPer < p.n)
+                        tma_store_2d(tmO, smem_u32(stage + h * kWideChunk), (n0 + c + h * kPer) * (int)sizeof(T), row0);
+                bulk_commit();
+            }
+            continue;
+        }
+        __syncwarp();
+        for (int i = lane; i < kWideChunks * kPer; i += 32) {
+            const int n = n0 + c + i, e = i % kPer;
+            if (n >= p.n) break;
+            const uint8_t* src = stage + i / kPer * kWideChunk;
+            for (int r = 0; r < rows && r < 32; ++r)
+                static_cast<T*>(p.out)[(int64_t)(row0 + r) * p.ldo + n] =
+                    reinterpret_cast<const T*>(src + r * 128 + (((e / kPiece) ^ r) & 7) * 16)[e % kPiece];
+        }
+        __syncwarp();
     }
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // Roles and bounded waits as above. Pairs: CTA 0 of the cluster issues the products for both;
@@ -534,7 +591,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, int dtype) {
 // epilogues hand accumulators back to it.
 template <int CG>
 __global__ void __launch_bounds__(kWideThreads, 1)
-matmul_fp8_wide_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmA, const TcArgs p) {
+matmul_fp8_wide_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmA,
+                       const __grid_constant__ CUtensorMap tmO, const TcArgs p) {
     constexpr int BT = 128 * CG;                             // tokens of a tile
     constexpr uint32_t kA = 128 * kBlock, kB = kWideN / CG * kBlock;
     extern __shared__ uint8_t smem_raw[];
@@ -542,9 +600,10 @@ matmul_fp8_wide_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_con
     const uint32_t base = (raw + 1023u) & ~1023u;
     uint8_t* const smem = smem_raw + (base - raw);
     const int stages = p.stages;
-    // [token slots | weight slots | scales | barriers | table], slots 1024-aligned
+    // [token slots | weight slots | output staging | scales | barriers | table], slots 1024-aligned
     const uint32_t ring_b = base + (uint32_t)stages * kA;
-    float* const scales = reinterpret_cast<float*>(smem + (size_t)stages * (kA + kB));
+    uint8_t* const staging = smem + (size_t)stages * (kA + kB);
+    float* const scales = reinterpret_cast<float*>(staging + kWideEpi * kWideStage);
     uint64_t* const full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(scales) + 2 * kWideScales);
     uint64_t* const empty = full + stages;
     uint64_t* const tfull = empty + stages;
@@ -609,10 +668,7 @@ matmul_fp8_wide_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_con
                     if (rank == 0) mbar_expect_tx(&full[st], CG * (kA + kB));
                     const uint32_t bar = CG == 2 ? mapa(smem_u32(&full[st]), 0) : smem_u32(&full[st]);
                     wide_load_2d<CG>(base + (uint32_t)st * kA, &tmA, bar, kb * kBlock, tl.row0 + (int)rank * 128);
-                    // 128 weight rows per box
-                    for (int h = 0; h < 2 / CG; ++h)
-                        wide_load_3d<CG>(ring_b + (uint32_t)st * kB + h * (128 * kBlock), &tmB, bar, kb * kBlock,
-                                         tl.n0 + ((int)rank + h) * 128, tl.expert);
+                    wide_load_3d<CG>(ring_b + (uint32_t)st * kB, &tmB, bar, kb * kBlock, tl.n0 + (int)rank * 128, tl.expert);
                 }
             }
             // the last load of every slot has landed before the CTA (or its pair) may exit
@@ -685,7 +741,8 @@ matmul_fp8_wide_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_con
     }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWideRegsMore));
-        const int q = warp & 3, half = (warp - 4) >> 2;      // TMEM lane quarter, weight block
+        const int q = warp & 3, grp = (warp - 4) >> 2;       // TMEM lane quarter, group of columns
+        const int half = grp * kWideCols / kBlock;           // their weight block
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
         const int tok = q * 32 + lane;
         float acc[kWideCols];
@@ -703,7 +760,7 @@ matmul_fp8_wide_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_con
                     break;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t src = tmem + lanes + (uint32_t)(ap.slot * kWideN + half * kWideCols);
+                const uint32_t src = tmem + lanes + (uint32_t)(ap.slot * kWideN + grp * kWideCols);
                 const float* sc = scales + cp.slot * (kWideScales / 4);
                 uint32_t r[2][32];
                 tmem_ld32_async(src, r[0]);
@@ -739,33 +796,13 @@ matmul_fp8_wide_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_con
                 }
             }
             if (failed) continue;
-            const int m = tok + (int)rank * 128, n0 = tl.n0 + half * kWideCols;
-            if (m < tl.rows) {
-                const int64_t at = (int64_t)(tl.row0 + m) * p.ldo + n0;
-                if (p.out_dtype == ENGINE_F32) {
-                    float* o = static_cast<float*>(p.out) + at;
-#pragma unroll
-                    for (int i = 0; i < kWideCols; i += 4)
-                        if (n0 + i + 4 <= p.n) *reinterpret_cast<float4*>(o + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
-                        else
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                if (n0 + i + j < p.n) o[i + j] = acc[i + j];
-                } else {
-                    uint16_t* o = static_cast<uint16_t*>(p.out) + at;
-#pragma unroll
-                    for (int i = 0; i < kWideCols; i += 8)
-                        if (n0 + i + 8 <= p.n)
-                            *reinterpret_cast<uint4*>(o + i) =
-                                make_uint4(pack2(acc[i], acc[i + 1], p.out_dtype), pack2(acc[i + 2], acc[i + 3], p.out_dtype),
-                                           pack2(acc[i + 4], acc[i + 5], p.out_dtype), pack2(acc[i + 6], acc[i + 7], p.out_dtype));
-                        else
-#pragma unroll
-                            for (int j = 0; j < 8; ++j)
-                                if (n0 + i + j < p.n) store_out(p.out, p.out_dtype, at + i + j, acc[i + j]);
-                }
-            }
+            uint8_t* const mine = staging + (warp - 4) * kWideStage;
+            const int row0 = q * 32 + (int)rank * 128, n0 = tl.n0 + grp * kWideCols;
+            if (p.out_dtype == ENGINE_BF16) wide_store<__nv_bfloat16>(p, &tmO, acc, mine, tl.row0 + row0, tl.rows - row0, n0);
+            else if (p.out_dtype == ENGINE_F16) wide_store<__half>(p, &tmO, acc, mine, tl.row0 + row0, tl.rows - row0, n0);
+            else wide_store<float>(p, &tmO, acc, mine, tl.row0 + row0, tl.rows - row0, n0);
         }
+        if (lane == 0) bulk_wait0();                         // the last stores have left shared memory
         if (p.offsets) {
             // rows before the first and after the last expert's
             const int lo = table[0], hi = table[2 * p.experts - 1];
@@ -840,10 +877,11 @@ void launch_tc(const TcArgs& args, int64_t grid, const CUtensorMap& tmB, const C
 }
 
 template <int CG>
-void launch_wide(const TcArgs& args, int64_t tiles, int sms, const CUtensorMap& tmB, const CUtensorMap& tmA, int device, cudaStream_t s) {
+void launch_wide(const TcArgs& args, int64_t tiles, int sms, const CUtensorMap& tmB, const CUtensorMap& tmA, const CUtensorMap& tmO, int device,
+                 cudaStream_t s) {
     TcArgs p = args;
     constexpr uint32_t stage = 128 * kBlock + kWideN / CG * kBlock;
-    const uint32_t fixed = 1024 + 2 * kWideScales + kBarrierBytes + p.table_bytes;
+    const uint32_t fixed = 1024 + kWideEpi * kWideStage + 2 * kWideScales + kBarrierBytes + p.table_bytes;
     p.stages = (int)std::min<uint32_t>(8, (227u * 1024u - fixed) / stage);
     static bool ready[64] = {};
     if (device >= 64 || !ready[device]) {
@@ -865,7 +903,50 @@ void launch_wide(const TcArgs& args, int64_t tiles, int sms, const CUtensorMap& 
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    PB_CUDA(cudaLaunchKernelEx(&cfg, matmul_fp8_wide_kernel<CG>, tmB, tmA, p));
+    PB_CUDA(cudaLaunchKernelEx(&cfg, matmul_fp8_wide_kernel<CG>, tmB, tmA, tmO, p));
+}
+
+}  // namespace
+
+namespace {
+
+// Which kernel and tile. wide: 0, or the CTAs per wide tile; else tiles of bt tokens with the
+// k-blocks of a tile split over `split` CTAs.
+struct Plan { int wide, bt, split; };
+
+// A k-block takes a CTA about as long whatever its tile holds (ns, one tile per SM, 4096 x 4096
+// weights: 16 tokens 330, 32: 380, 64: 430, 128: 490; a wide tile 520), so what counts is how
+// many k-blocks the busiest CTA gets. With one weight all shapes are known and the
+// smallest product of waves, k-blocks per CTA and those times wins. Measured (us, m x n x
+// k): 8 x 4096 x 4096: 16 tokens over 4 CTAs 8.6, over 2 12.9, over 1 16.4; 333 x 1201 x 2000:
+// 32 tokens 11.3, 64: 13.1, wide 20; 512 x 4096 x 4096: wide 22.3, 128 22.7, 64 35; 2048 x 4096
+// x 4096: wide 41, 128 74. Pairs where single wide tiles take more than a wave: 8192 x
+// 8192 x 4096 267 against 277.
+Plan plan_matmul(const MatmulFp8Args& g, int64_t experts, int sms) {
+    if (g.offsets) {
+        // The experts' shares are on the GPU; what is known is the average. Tiles about twice
+        // as wide as that hold most experts' rows at once. Measured (us, 64 experts, 2048 x 2048): 4 rows
+        // each: 16 tokens 52.5, 32: 53.8, wide 55.7; 16 rows: 32: 56.1, 64: 63.1, wide 66.4, 16: 70.8; 32 rows: 64: 65.0,
+        // wide 68.8, 128: 71.8; 64 rows: wide 71.3, 128: 76.1, 64: 103.
+        const int64_t r = g.m / experts;
+        return r <= 6 ? Plan{0, 16, 1} : r <= 20 ? Plan{0, 32, 1} : r <= 48 ? Plan{0, 64, 1} : Plan{1, 128, 1};
+    }
+    const int64_t nkb = (g.k + kBlock - 1) / kBlock, n_tiles = (g.n + kTileN - 1) / kTileN;
+    auto waves = [&](int64_t tiles) { return (tiles + sms - 1) / sms; };
+    const int64_t wide_tiles = (g.m + 127) / 128 * ((g.n + kWideN - 1) / kWideN);
+    Plan best{wide_tiles > sms ? 2 : 1, 128, 1};
+    double least = (double)waves(wide_tiles) * nkb * 520;
+    const int bts[] = {128, 64, 32, 16}, ns[] = {490, 430, 380, 330};
+    for (int i = 0; i < 4; ++i) {
+        const int64_t tiles = (g.m + bts[i] - 1) / bts[i] * n_tiles;
+        for (int split = 1; split <= 8; split *= 2) {
+            if (split > 1 && (tiles * split > sms || nkb < 2 * split)) break;
+            // joining the sums of a split costs about two k-blocks
+            const double t = ((double)waves(tiles) * ((nkb + split - 1) / split) + (split > 1 ? 2 : 0)) * ns[i];
+            if (t < least) { least = t; best = Plan{0, bts[i], split}; }
+        }
+    }
+    return best;
 }
 
 }  // namespace
@@ -928,11 +1009,9 @@ void launch_matmul_fp8(const MatmulFp8Args& g, cudaStream_t s) {
     p.wait_limit = 1000000000LL;
     p.split = 1;
 
-    // Tokens of a tile: the smallest width that holds the rows (an expert's average), so that
-    // few tokens do not pay for a wide tile's empty columns.
-    const int64_t rows = g.offsets ? (g.m + experts - 1) / experts : g.m;
-    const int wide = (getenv("WIDE") ? atoi(getenv("WIDE")) : 2) * (rows > 128 && reinterpret_cast<uintptr_t>(g.out) % 16 == 0 && g.ldo * (g.out_dtype == ENGINE_F32 ? 4 : 2) % 16 == 0);
-    const int bt = wide ? 128 : rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+    const Plan plan = plan_matmul(g, experts, sms);
+    const int wide = plan.wide, bt = wide ? 128 : plan.bt;
+    p.wide_out = reinterpret_cast<uintptr_t>(g.out) % 16 == 0 && (g.m <= 1 || g.ldo * (g.out_dtype == ENGINE_F32 ? 4 : 2) % 16 == 0);
     const int tokens = wide ? 128 * wide : bt;
     p.m_tiles = (int)((g.m + tokens - 1) / tokens);
 
@@ -940,36 +1019,38 @@ void launch_matmul_fp8(const MatmulFp8Args& g, cudaStream_t s) {
     {
         const uint64_t dims[2] = {(uint64_t)g.k, (uint64_t)g.m}, st[1] = {(uint64_t)lda};
         const uint32_t box[2] = {kBlock, (uint32_t)bt};
-        if (!encode_box_map(&tmA, 1, 2, a, dims, st, box, true)) fail(ENGINE_ERR_INVALID_ARG, "matmul_fp8: tensor map of a refused");
+        if (!encode_box_map(&tmA, 1, 2, a, dims, st, box, 128)) fail(ENGINE_ERR_INVALID_ARG, "matmul_fp8: tensor map of a refused");
     }
     {
         const uint64_t dims[3] = {(uint64_t)g.k, (uint64_t)g.n, (uint64_t)experts}, st[2] = {(uint64_t)ldb, (uint64_t)b_expert};
-        const uint32_t box[3] = {kBlock, kTileN, 1};
-        if (!encode_box_map(&tmB, 1, 3, b, dims, st, box, true)) fail(ENGINE_ERR_INVALID_ARG, "matmul_fp8: tensor map of b refused");
+        const uint32_t box[3] = {kBlock, (uint32_t)(wide == 1 ? kWideN : kTileN), 1};
+        if (!encode_box_map(&tmB, 1, 3, b, dims, st, box, 128)) fail(ENGINE_ERR_INVALID_ARG, "matmul_fp8: tensor map of b refused");
     }
 
     if (wide) {
         p.n_tiles = (int)((g.n + kWideN - 1) / kWideN);
         const int64_t tiles = (g.offsets ? std::min<int64_t>(g.m, experts + g.m / tokens) : p.m_tiles) * p.n_tiles;
-        if (wide == 1) launch_wide<1>(p, tiles, sms, tmB, tmA, device, s);
-        else launch_wide<2>(p, tiles, sms, tmB, tmA, device, s);
+        CUtensorMap tmO = tmA;
+        if (p.wide_out) {
+            const uint64_t e = g.out_dtype == ENGINE_F32 ? 4 : 2;
+            const uint64_t dims[2] = {(uint64_t)g.n * e, (uint64_t)g.m}, st[1] = {(uint64_t)(g.m > 1 ? g.ldo : (g.n + 15) / 16 * 16) * e};
+            const uint32_t box[2] = {128, 32};
+            if (!encode_box_map(&tmO, 1, 2, g.out, dims, st, box, 128)) fail(ENGINE_ERR_INVALID_ARG, "matmul_fp8: tensor map of the output refused");
+        }
+        if (wide == 1) launch_wide<1>(p, tiles, sms, tmB, tmA, tmO, device, s);
+        else launch_wide<2>(p, tiles, sms, tmB, tmA, tmO, device, s);
         return;
     }
     // Token tiles there can be at most: one per expert with rows, and one per full tile.
     const int64_t tiles = (g.offsets ? std::min<int64_t>(g.m, experts + g.m / bt) : p.m_tiles) * p.n_tiles;
-    // Few tiles: a cluster of 2, 4 or 8 CTAs per tile, as long as each still gets two k-blocks
-    // and the clusters fit the SMs at once.
-    int split = 1;
-    if (!g.offsets && bt <= 128)
-        while (split < 8 && tiles * split * 2 <= sms && p.nkb >= split * 4) split *= 2;
+    const int split = plan.split;
     p.split = split;
     const int64_t grid = split > 1 ? tiles * split : std::min<int64_t>(tiles, sms);
     switch (bt) {
         case 16: split > 1 ? launch_tc<16, true>(p, grid, tmB, tmA, device, s) : launch_tc<16, false>(p, grid, tmB, tmA, device, s); break;
         case 32: split > 1 ? launch_tc<32, true>(p, grid, tmB, tmA, device, s) : launch_tc<32, false>(p, grid, tmB, tmA, device, s); break;
         case 64: split > 1 ? launch_tc<64, true>(p, grid, tmB, tmA, device, s) : launch_tc<64, false>(p, grid, tmB, tmA, device, s); break;
-        case 128: split > 1 ? launch_tc<128, true>(p, grid, tmB, tmA, device, s) : launch_tc<128, false>(p, grid, tmB, tmA, device, s); break;
-        default: launch_tc<256, false>(p, grid, tmB, tmA, device, s); break;
+        default: split > 1 ? launch_tc<128, true>(p, grid, tmB, tmA, device, s) : launch_tc<128, false>(p, grid, tmB, tmA, device, s); break;
     }
 }
 
