@@ -4,22 +4,29 @@ The library is built in-tree (objects under pdefa_b200/_build, the shared object
 under pdefa_b200/lib) for sm_100a only. Only the C-ABI entry points are exported
 (-fvisibility=hidden + explicit default visibility on the API declarations).
 
+Where torch is installed, lib/lm_torch.so (pdefa_b200/torch_ext) is built too: the
+binding of the language-model operators for torch tensors.
+
 Usage: python -m pdefa_b200.build [--force] [--jobs N]
 """
 from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 SRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIB_DIR, "libpdefa_native.so")
+TORCH_SRC = os.path.join(HERE, "torch_ext", "lm_torch.cpp")
+TORCH_LIB = os.path.join(LIB_DIR, "lm_torch.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -55,13 +62,35 @@ def compile_one(src: str, force: bool) -> str:
     return obj
 
 
+def build_torch_binding(force: bool) -> None:
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not spec.origin:
+        return
+    if (not force and os.path.exists(TORCH_LIB)
+            and os.path.getmtime(TORCH_LIB) >= max(os.path.getmtime(TORCH_SRC), _newest_header())):
+        return
+    root = os.path.dirname(spec.origin)
+    cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_paths()["include"], cuda]
+    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", *("-I" + i for i in inc), TORCH_SRC,
+           "-o", TORCH_LIB + ".tmp", "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
+           "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"torch binding failed:\n{r.stdout}\n{r.stderr}")
+    os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
+
+
 def build(force: bool = False, jobs: int = 0) -> str:
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(LIB_DIR, exist_ok=True)
     srcs = sources()
-    jobs = jobs or min(len(srcs), os.cpu_count() or 4)
+    jobs = jobs or min(len(srcs) + 1, os.cpu_count() or 4)
     with cf.ThreadPoolExecutor(jobs) as ex:
+        binding = ex.submit(build_torch_binding, force)
         objs = list(ex.map(lambda s: compile_one(s, force), srcs))
+        binding.result()
     if (force or not os.path.exists(LIB)
             or max(os.path.getmtime(o) for o in objs) > os.path.getmtime(LIB)):
         cmd = [nvcc(), "-shared", *ARCH, "-cudart", "static", "-o", LIB + ".tmp", *objs, "-lpthread", "-ldl", "-lrt", "-lz"]
