@@ -11,12 +11,13 @@
 // TMEM columns), so a handful of tokens costs a narrow tile and not 128 padded rows.
 // Scales change with every 128 k, so an accumulator cannot run through K on the tensor
 // core: each k-block (one 128-byte swizzled row per operand row, four instructions of
-// K = 32) goes into a fresh TMEM buffer, and the epilogue warps add buffer * scale to
+// K = 32) goes into a fresh TMEM accumulator, and the epilogue warps add buffer * scale to
 // 32-bit sums in registers, while the tensor core fills the next buffer. The tile's
 // weight rows share one scale per k-block (tiles start at multiples of 128), the
 // tokens have one each; their products come from shared memory as one broadcast load
 // per four columns, and the sum is one packed fp32x2 multiply-add per two columns.
 #include <algorithm>
+#include <atomic>
 #include <cuda.h>
 #include <cuda_fp16.h>
 
@@ -31,7 +32,7 @@ namespace {
 constexpr int kBlock = 128;             // k per scale, and bytes of an operand row per stage
 constexpr int kTileN = 128;             // weight rows of a tile
 constexpr int kScaleChunk = 8;          // k-blocks of scales staged at a time (one 32-byte sector per token)
-constexpr uint32_t kABytes = kTileN * kBlock;
+constexpr uint32_t kABytes = 2 * kTileN * kBlock;   // weights of a stage
 constexpr uint32_t kBarrierBytes = 512;
 
 struct TcArgs {
@@ -57,10 +58,10 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
-    float v;
-    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}"
-                 : "=f"(v) : "r"(addr), "r"(rank) : "memory");
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr, uint32_t rank) {
+    float4 v;
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\tld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr), "r"(rank) : "memory");
     return v;
 }
 
@@ -69,10 +70,8 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, long l
     return __all_sync(~0u, mbar_wait_bounded(bar, parity, limit));
 }
 
-// One k-block: four K = 32 products into a fresh accumulator, then a commit to the ring
-// slot's barrier, which tells the loads that the slot is free and the epilogue that the
-// accumulator is full.
-__device__ __forceinline__ void mma_kblock(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint64_t* done) {
+// One k-block: four K = 32 products into a fresh accumulator.
+__device__ __forceinline__ void mma_kblock(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc) {
     asm volatile(
         "{\n\t.reg .pred pf, pt;\n\t.reg .b64 a1, b1, a2, b2, a3, b3;\n\t"
         "setp.ne.u32 pf, 0, 0;\n\tsetp.eq.u32 pt, 0, 0;\n\t"
@@ -81,9 +80,8 @@ __device__ __forceinline__ void mma_kblock(uint32_t d, uint64_t da, uint64_t db,
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, pf;\n\t"
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a1, b1, %3, pt;\n\t"
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a2, b2, %3, pt;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a3, b3, %3, pt;\n\t"
-        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%4];\n\t}"
-        ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(smem_u32(done))
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a3, b3, %3, pt;\n\t}"
+        ::"r"(d), "l"(da), "l"(db), "r"(idesc)
         : "memory");
 }
 
@@ -92,9 +90,9 @@ struct Shape {
     static constexpr int kEpi = BT >= 128 ? 8 : 4;                  // epilogue warps
     static constexpr int kThreads = 128 + 32 * kEpi;
     static constexpr int kCols = BT * 4 / kEpi;                     // columns of an epilogue thread
-    static constexpr int kBufs = 4;                                 // TMEM accumulators
-    static constexpr int kTmemCols = kBufs * BT;                    // 64 .. 512
-    static constexpr uint32_t kBBytes = BT * kBlock;
+    static constexpr int kBufs = 2;                                 // TMEM buffers, of two accumulators each
+    static constexpr int kTmemCols = kBufs * 2 * BT;                // 64 .. 512
+    static constexpr uint32_t kBBytes = 2 * BT * kBlock;            // tokens of a stage
     static constexpr uint32_t kScaleBytes = kScaleChunk * BT * 4;   // of one of two chunks
 };
 
@@ -175,6 +173,31 @@ __device__ __forceinline__ void store_out(void* out, int dtype, int64_t i, float
     else static_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
 }
 
+// Four columns of a row, n a multiple of 4.
+__device__ __forceinline__ void store_out4(const TcArgs& p, int row, int n, float4 v) {
+    const int64_t at = (int64_t)row * p.ldo + n;
+    if (p.wide_out && n + 4 <= p.n) {
+        if (p.out_dtype == ENGINE_F32) {
+            *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = v;
+        } else {
+            uint2 q;
+            if (p.out_dtype == ENGINE_F16) {
+                const __half2 lo = __floats2half2_rn(v.x, v.y), hi = __floats2half2_rn(v.z, v.w);
+                q = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+            } else {
+                const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+                q = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+            }
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = q;
+        }
+        return;
+    }
+    const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (n + i < p.n) store_out(p.out, p.out_dtype, at + i, e[i]);
+}
+
 // Roles: warps 0 and 3 bring operands (TMA), warp 1 issues the products and owns TMEM, warp 2
 // brings scales, warps 4 and up are the epilogue. Every wait is bounded; one that runs
 // out records a code in the device's error word and ends its role, after which the
@@ -228,12 +251,13 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
     const int token_tiles = *tile_count;
     const int64_t total = (int64_t)token_tiles * p.n_tiles;
 
-    // this CTA's tiles and, of each, its k-blocks
+    // this CTA's tiles and, of each, its pairs of k-blocks (the last one's second may be past the end: zeros)
     const uint32_t rank = SPLIT ? cluster_rank() : 0;
     const int64_t t0 = SPLIT ? blockIdx.x / p.split : blockIdx.x;
     const int64_t tstep = SPLIT ? total : gridDim.x;        // SPLIT: one tile per cluster
-    const int kb0 = SPLIT ? (int)((int64_t)p.nkb * rank / p.split) : 0;
-    const int kb1 = SPLIT ? (int)((int64_t)p.nkb * (rank + 1) / p.split) : p.nkb;
+    const int pairs = (p.nkb + 1) / 2;
+    const int pr0 = SPLIT ? (int)((int64_t)pairs * rank / p.split) : 0;
+    const int pr1 = SPLIT ? (int)((int64_t)pairs * (rank + 1) / p.split) : pairs;
 
     float acc[S::kCols];
     Tile mine{0, 0, 0, 0};
@@ -248,7 +272,7 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
             int64_t it = 0;
             for (int64_t t = t0; t < total && !failed; t += tstep) {
                 const Tile tl = tile_of<BT, kTileN>(p, table, token_tiles, t);
-                for (int kb = kb0; kb < kb1; ++kb) {
+                for (int pr = pr0; pr < pr1; ++pr) {
                     const int st = rp.slot;
                     if (rp.wrapped && !mbar_wait_bounded(&done[st], rp.phase ^ 1u, p.wait_limit)) {
                         atomicExch(p.err, 21);
@@ -258,8 +282,11 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
                     rp.next(stages);
                     ++it;
                     mbar_expect_tx(&full[st], weights ? kABytes : S::kBBytes);
-                    if (weights) tma_load_3d(base + (uint32_t)st * kABytes, &tmB, &full[st], kb * kBlock, tl.n0, tl.expert);
-                    else tma_load_2d(ring_b + (uint32_t)st * S::kBBytes, &tmA, &full[st], kb * kBlock, tl.row0);
+                    for (int h = 0; h < 2; ++h) {
+                        const int k = (2 * pr + h) * kBlock;
+                        if (weights) tma_load_3d(base + (uint32_t)st * kABytes + h * (kABytes / 2), &tmB, &full[st], k, tl.n0, tl.expert);
+                        else tma_load_2d(ring_b + (uint32_t)st * S::kBBytes + h * (S::kBBytes / 2), &tmA, &full[st], k, tl.row0);
+                    }
                 }
             }
             // the last load of every slot has landed before the CTA may exit
@@ -273,7 +300,7 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
             const uint32_t idesc = (1u << 4) | ((uint32_t)(BT >> 3) << 17) | ((uint32_t)(kTileN >> 4) << 24);
             RingPos rp, ap;
             for (int64_t t = t0; t < total && !failed; t += tstep) {
-                for (int kb = kb0; kb < kb1; ++kb) {
+                for (int pr = pr0; pr < pr1; ++pr) {
                     const int st = rp.slot, buf = ap.slot;
                     if ((ap.wrapped && !mbar_wait_bounded(&tempty[buf], ap.phase ^ 1u, p.wait_limit)) ||
                         !mbar_wait_bounded(&full[st], rp.phase, p.wait_limit)) {
@@ -282,8 +309,13 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
                         break;
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    mma_kblock(tmem + (uint32_t)(buf * BT), make_smem_desc(base + (uint32_t)st * kABytes, 128),
-                               make_smem_desc(ring_b + (uint32_t)st * S::kBBytes, 128), idesc, &done[st]);
+                    const uint64_t da = make_smem_desc(base + (uint32_t)st * kABytes, 128);
+                    const uint64_t db = make_smem_desc(ring_b + (uint32_t)st * S::kBBytes, 128);
+                    const uint32_t d = tmem + (uint32_t)(buf * 2 * BT);
+                    // the second halves, in the descriptors' units of 16 bytes
+                    mma_kblock(d, da, db, idesc);
+                    mma_kblock(d + BT, da + (kABytes / 2 >> 4), db + (S::kBBytes / 2 >> 4), idesc);
+                    umma_commit(&done[st]);
                     rp.next(stages);
                     ap.next(S::kBufs);
                 }
@@ -298,7 +330,8 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
             const Tile tl = tile_of<BT, kTileN>(p, table, token_tiles, t);
             const float* sa = p.sa + (int64_t)tl.row0 * p.lda_scales;
             const float* sb = p.sb + tl.expert * p.sb_expert + (tl.n0 / kTileN) * p.ldb_scales;
-            for (int kc = kb0; kc < kb1 && !failed; kc += kScaleChunk) {
+            for (int kc = 2 * pr0; kc < 2 * pr1 && !failed; kc += kScaleChunk) {
+                const int kb1 = min(2 * pr1, p.nkb);
                 float w[kScaleChunk];
 #pragma unroll
                 for (int j = 0; j < kScaleChunk; ++j) w[j] = kc + j < kb1 ? __ldg(sb + kc + j) : 0.0f;
@@ -332,8 +365,8 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
             mine = tile_of<BT, kTileN>(p, table, token_tiles, t);
 #pragma unroll
             for (int i = 0; i < S::kCols; ++i) acc[i] = 0.0f;
-            for (int kb = kb0; kb < kb1; ++kb) {
-                const int in_chunk = (kb - kb0) % kScaleChunk;
+            for (int pr = pr0; pr < pr1; ++pr) {
+                const int in_chunk = 2 * (pr - pr0) % kScaleChunk;
                 if ((in_chunk == 0 && !warp_wait(&sfull[cp.slot], cp.phase, p.wait_limit)) ||
                     !warp_wait(&done[rp.slot], rp.phase, p.wait_limit)) {
                     if (lane == 0) atomicExch(p.err, 25);
@@ -341,14 +374,15 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
                     break;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t src = tmem + lanes + (uint32_t)(ap.slot * BT + c0);
-                const float4* sc = reinterpret_cast<const float4*>(scales + cp.slot * (kScaleChunk * BT) + in_chunk * BT + c0);
+                const uint32_t src = tmem + lanes + (uint32_t)(ap.slot * 2 * BT + c0);
+                const float* sc = scales + cp.slot * (kScaleChunk * BT) + in_chunk * BT + c0;
+                constexpr int kChunks = S::kCols / 16;               // per k-block
                 uint32_t r[2][16];
                 tmem_ld16_async(src, r[0]);
 #pragma unroll
-                for (int c = 0; c < S::kCols / 16; ++c) {
+                for (int c = 0; c < 2 * kChunks; ++c) {
                     tmem_wait_ld();
-                    if (c + 1 < S::kCols / 16) tmem_ld16_async(src + (c + 1) * 16, r[(c + 1) & 1]);
+                    if (c + 1 < 2 * kChunks) tmem_ld16_async(src + (c + 1) / kChunks * BT + (c + 1) % kChunks * 16, r[(c + 1) & 1]);
                     else {
                         // everything is in registers: the tensor core may refill the buffer
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -356,10 +390,11 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
                         if (lane == 0) mbar_arrive(&tempty[ap.slot]);
                     }
                     const uint32_t(&v)[16] = r[c & 1];
+                    const float4* s4p = reinterpret_cast<const float4*>(sc + c / kChunks * BT + c % kChunks * 16);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const float4 s4 = sc[c * 4 + j];
-                        float* d = acc + c * 16 + j * 4;
+                        const float4 s4 = s4p[j];
+                        float* d = acc + c % kChunks * 16 + j * 4;
                         const float2 lo = __ffma2_rn(make_float2(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1])),
                                                      make_float2(s4.x, s4.y), make_float2(d[0], d[1]));
                         const float2 hi = __ffma2_rn(make_float2(__uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3])),
@@ -369,7 +404,7 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
                 }
                 rp.next(stages);
                 ap.next(S::kBufs);
-                if (in_chunk == kScaleChunk - 1 || kb == kb1 - 1) {
+                if (in_chunk == kScaleChunk - 2 || pr == pr1 - 1) {
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sempty[cp.slot]);
                     cp.next(2);
@@ -406,13 +441,20 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
         __syncwarp();
         cluster_sync();
         if (warp >= 4 && !failed) {
-            const int tid = threadIdx.x - 128;
-            const int per = BT / p.split, n = mine.n0 + (tid & 127);
-            for (int j = (int)rank * per + (tid >> 7); j < ((int)rank + 1) * per; j += S::kEpi / 4) {
+            // each CTA joins its share of the tokens, four weight rows per thread and load
+            const int per = BT / p.split;
+            for (int i = threadIdx.x - 128; i < per * (kTileN / 4); i += 32 * S::kEpi) {
+                const int j = (int)rank * per + i / (kTileN / 4), n = mine.n0 + i % (kTileN / 4) * 4;
                 if (j >= mine.rows || n >= p.n) continue;
-                float sum = 0.0f;
-                for (int c = 0; c < p.split; ++c) sum += ld_cluster(smem_u32(part + j * kTileN + (tid & 127)), c);
-                store_out(p.out, p.out_dtype, (int64_t)(mine.row0 + j) * p.ldo + n, sum);
+                const uint32_t at = smem_u32(part + j * kTileN + i % (kTileN / 4) * 4);
+                float4 v[8], sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    if (c < p.split) v[c] = ld_cluster(at, c);
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    if (c < p.split) { sum.x += v[c].x; sum.y += v[c].y; sum.z += v[c].z; sum.w += v[c].w; }
+                store_out4(p, mine.row0 + j, n, sum);
             }
         }
         __syncwarp();
@@ -850,13 +892,16 @@ struct PoolBuffer {
     ~PoolBuffer() { if (p) cudaFreeAsync(p, s); }
 };
 
+// The kernel with its shared memory, launched on a grid of clusters of `split` CTAs, or asked how
+// many of these clusters the device holds at once.
 template <int BT, bool SPLIT>
-void launch_tc(const TcArgs& args, int64_t grid, const CUtensorMap& tmB, const CUtensorMap& tmA, int device, cudaStream_t s) {
+int tc_kernel(const TcArgs& args, int64_t grid, int split, const CUtensorMap* tmB, const CUtensorMap* tmA, int device,
+              cudaStream_t s) {
     using S = Shape<BT>;
     TcArgs p = args;
     const uint32_t fixed = 1024 + 2 * S::kScaleBytes + kBarrierBytes + p.table_bytes;
-    p.stages = (int)std::min<uint32_t>(12, (227u * 1024u - fixed) / (kABytes + S::kBBytes));
-    const size_t smem = fixed + (size_t)p.stages * (kABytes + S::kBBytes);
+    p.stages = (int)((227u * 1024u - fixed) / (kABytes + S::kBBytes));       // 3 to 6
+    p.split = split;
     static bool ready[64] = {};
     if (device >= 64 || !ready[device]) {
         PB_CUDA(cudaFuncSetAttribute(matmul_fp8_kernel<BT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
@@ -865,15 +910,34 @@ void launch_tc(const TcArgs& args, int64_t grid, const CUtensorMap& tmB, const C
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(S::kThreads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = fixed + (size_t)p.stages * (kABytes + S::kBBytes);
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)p.split;
+    at[0].val.clusterDim.x = (unsigned)split;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = SPLIT ? 1 : 0;
-    PB_CUDA(cudaLaunchKernelEx(&cfg, matmul_fp8_kernel<BT, SPLIT>, tmB, tmA, p));
+    if (!tmB) {
+        int n = 0;
+        PB_CUDA(cudaOccupancyMaxActiveClusters(&n, matmul_fp8_kernel<BT, SPLIT>, &cfg));
+        return n;
+    }
+    PB_CUDA(cudaLaunchKernelEx(&cfg, matmul_fp8_kernel<BT, SPLIT>, *tmB, *tmA, p));
+    return 0;
+}
+
+// Clusters of `split` CTAs of the narrow kernels that run at once. (They stay within a GPC,
+// so it is fewer than the SMs make: 16 clusters of 8 took two waves.)
+int64_t clusters_at_once(int split, int device) {
+    static std::atomic<int> known[64][4] = {};
+    const int i = split == 2 ? 0 : split == 4 ? 1 : 2;
+    int n = device < 64 ? known[device][i].load() : 0;
+    if (!n) {
+        n = tc_kernel<16, true>(TcArgs{}, split, split, nullptr, nullptr, device, nullptr);
+        if (device < 64) known[device][i].store(n);
+    }
+    return n;
 }
 
 template <int CG>
@@ -914,15 +978,16 @@ namespace {
 // k-blocks of a tile split over `split` CTAs.
 struct Plan { int wide, bt, split; };
 
-// A k-block takes a CTA about as long whatever its tile holds (ns, one tile per SM, 4096 x 4096
-// weights: 16 tokens 330, 32: 380, 64: 430, 128: 490; a wide tile 520), so what counts is how
-// many k-blocks the busiest CTA gets. With one weight all shapes are known and the
-// smallest product of waves, k-blocks per CTA and those times wins. Measured (us, m x n x
-// k): 8 x 4096 x 4096: 16 tokens over 4 CTAs 8.6, over 2 12.9, over 1 16.4; 333 x 1201 x 2000:
-// 32 tokens 11.3, 64: 13.1, wide 20; 512 x 4096 x 4096: wide 22.3, 128 22.7, 64 35; 2048 x 4096
-// x 4096: wide 41, 128 74. Pairs where single wide tiles take more than a wave: 8192 x
-// 8192 x 4096 267 against 277.
-Plan plan_matmul(const MatmulFp8Args& g, int64_t experts, int sms) {
+// A k-block takes a CTA nearly as long whatever its tile holds, so what counts is how many of
+// them the busiest CTA gets. With one weight all shapes are known: of every tile the time of
+// the busiest CTA is waves * (k-blocks * time of one + time to store the tile), or with a split
+// the k-blocks' and the joining's, and the least wins. The times (us) are fits to a sweep on
+// a B200, which they meet within 10%. Measured, m x n x k: 16 x 4096 x 4096: 16 tokens over 4
+// CTAs 7.5, over 2 9.1, over 1 12.3; 64 x 4096 x 4096: 64 over 4 8.9, 32 over 2 10.2, 16 over 1 12.6;
+// 333 x 1201 x 2000: 32 over 1 9.8, 64 over 2 9.9, 128 over 4 11.0, wide 19; 512 x 4096 x 4096: 128
+// over 1 19.0, wide 22.2, 64 27.4; 800 x 4096 x 4096: wide 22.9, 128 33. Pairs where wide tiles
+// are more than one wave: 8192 x 8192 x 4096 267 against 277.
+Plan plan_matmul(const MatmulFp8Args& g, int64_t experts, int sms, int device) {
     if (g.offsets) {
         // The experts' shares are on the GPU; what is known is the average. Tiles about twice
         // as wide as that hold most experts' rows at once. Measured (us, 64 experts, 2048 x 2048): 4 rows
@@ -935,15 +1000,15 @@ Plan plan_matmul(const MatmulFp8Args& g, int64_t experts, int sms) {
     auto waves = [&](int64_t tiles) { return (tiles + sms - 1) / sms; };
     const int64_t wide_tiles = (g.m + 127) / 128 * ((g.n + kWideN - 1) / kWideN);
     Plan best{wide_tiles > sms ? 2 : 1, 128, 1};
-    double least = (double)waves(wide_tiles) * nkb * 520;
-    const int bts[] = {128, 64, 32, 16}, ns[] = {490, 430, 380, 330};
-    for (int i = 0; i < 4; ++i) {
-        const int64_t tiles = (g.m + bts[i] - 1) / bts[i] * n_tiles;
+    double least = (double)waves(wide_tiles) * (nkb * 0.5 + 1.2);
+    static const struct { int bt; double block, store, join; } kTiles[] = {
+        {128, 0.33, 2.6, 5.2}, {64, 0.27, 2.1, 2.6}, {32, 0.26, 0.9, 1.7}, {16, 0.245, 0.1, 1.2}};
+    for (const auto& c : kTiles) {
+        const int64_t tiles = (g.m + c.bt - 1) / c.bt * n_tiles;
         for (int split = 1; split <= 8; split *= 2) {
-            if (split > 1 && (tiles * split > sms || nkb < 2 * split)) break;
-            // joining the sums of a split costs about two k-blocks
-            const double t = ((double)waves(tiles) * ((nkb + split - 1) / split) + (split > 1 ? 2 : 0)) * ns[i];
-            if (t < least) { least = t; best = Plan{0, bts[i], split}; }
+            if (split > 1 && (nkb < 2 * split || tiles * split > sms || tiles > clusters_at_once(split, device))) break;
+            const double t = split == 1 ? (double)waves(tiles) * (nkb * c.block + c.store) : (double)((nkb + split - 1) / split) * c.block + c.join;
+            if (t < least) { least = t; best = Plan{0, c.bt, split}; }
         }
     }
     return best;
@@ -1007,9 +1072,8 @@ void launch_matmul_fp8(const MatmulFp8Args& g, cudaStream_t s) {
     p.table_bytes = g.offsets ? (uint32_t)(12 * experts + 15) & ~15u : 0;
     p.err = device_error_word(device);
     p.wait_limit = 1000000000LL;
-    p.split = 1;
 
-    const Plan plan = plan_matmul(g, experts, sms);
+    const Plan plan = plan_matmul(g, experts, sms, device);
     const int wide = plan.wide, bt = wide ? 128 : plan.bt;
     p.wide_out = reinterpret_cast<uintptr_t>(g.out) % 16 == 0 && (g.m <= 1 || g.ldo * (g.out_dtype == ENGINE_F32 ? 4 : 2) % 16 == 0);
     const int tokens = wide ? 128 * wide : bt;
@@ -1044,13 +1108,12 @@ void launch_matmul_fp8(const MatmulFp8Args& g, cudaStream_t s) {
     // Token tiles there can be at most: one per expert with rows, and one per full tile.
     const int64_t tiles = (g.offsets ? std::min<int64_t>(g.m, experts + g.m / bt) : p.m_tiles) * p.n_tiles;
     const int split = plan.split;
-    p.split = split;
     const int64_t grid = split > 1 ? tiles * split : std::min<int64_t>(tiles, sms);
     switch (bt) {
-        case 16: split > 1 ? launch_tc<16, true>(p, grid, tmB, tmA, device, s) : launch_tc<16, false>(p, grid, tmB, tmA, device, s); break;
-        case 32: split > 1 ? launch_tc<32, true>(p, grid, tmB, tmA, device, s) : launch_tc<32, false>(p, grid, tmB, tmA, device, s); break;
-        case 64: split > 1 ? launch_tc<64, true>(p, grid, tmB, tmA, device, s) : launch_tc<64, false>(p, grid, tmB, tmA, device, s); break;
-        default: split > 1 ? launch_tc<128, true>(p, grid, tmB, tmA, device, s) : launch_tc<128, false>(p, grid, tmB, tmA, device, s); break;
+        case 16: split > 1 ? tc_kernel<16, true>(p, grid, split, &tmB, &tmA, device, s) : tc_kernel<16, false>(p, grid, 1, &tmB, &tmA, device, s); break;
+        case 32: split > 1 ? tc_kernel<32, true>(p, grid, split, &tmB, &tmA, device, s) : tc_kernel<32, false>(p, grid, 1, &tmB, &tmA, device, s); break;
+        case 64: split > 1 ? tc_kernel<64, true>(p, grid, split, &tmB, &tmA, device, s) : tc_kernel<64, false>(p, grid, 1, &tmB, &tmA, device, s); break;
+        default: split > 1 ? tc_kernel<128, true>(p, grid, split, &tmB, &tmA, device, s) : tc_kernel<128, false>(p, grid, 1, &tmB, &tmA, device, s); break;
     }
 }
 
