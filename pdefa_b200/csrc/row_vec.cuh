@@ -35,11 +35,14 @@ struct RowLoader {
         words = (int)(off >> 2);
         bits = (int)(off & 3) * 8;
     }
-    // vectors before this one are aligned and whole
-    __device__ __forceinline__ uint32_t easy() const { return (words | bits) == 0 ? n / kPer : 0; }
+    __device__ __forceinline__ bool aligned() const { return (words | bits) == 0; }
+    __device__ __forceinline__ uint32_t whole() const { return n / kPer; }      // vectors without elements past the end
+    // vectors 1 .. inner() - 1 have both their aligned ones inside the row
+    __device__ __forceinline__ uint32_t inner() const { return n / kPer > 0 ? n / kPer - 1 : 0; }
+    __device__ __forceinline__ uint4 shifted(const uint4& lo, const uint4& hi) const { return shift_pair(lo, hi, words, bits); }
     __device__ __forceinline__ uint4 operator()(uint32_t v) const {
         const uint32_t i = v * kPer;
-        if ((words | bits) == 0 && i + kPer <= n) return base[v];
+        if (aligned() && i + kPer <= n) return base[v];
         // both vectors lie inside the row unless v is its first or its last
         if (v > 0 && i + 2 * kPer <= n) return shift_pair(base[v], base[v + 1], words, bits);
         uint32_t w[4];

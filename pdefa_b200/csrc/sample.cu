@@ -472,25 +472,45 @@ sample_cluster_kernel(SampleArgs a, int shift, int ctas) {
     float top;
     {
         uint4 m = vec_none<T>();
-        const uint32_t easy = min(all, max(load.easy(), v0) - v0);
         const uint4* src = load.base + v0;
         auto put = [&](uint32_t v, uint4 q) {
             q = vec_max_of<T>(q, vec_none<T>());        // NaN -> -inf
             slice[v] = q;
             m = vec_max_of<T>(m, q);
         };
-        uint32_t v = tid;
-        for (; v + 7 * kSlice < easy; v += 8 * kSlice) {
-            uint4 q[8];
+        // Several loads per thread are under way before the first is used: 8 vectors of an aligned
+        // row, or 4 pairs of one that is not. The row's first and last vectors go one by one.
+        uint32_t rest;
+        if (load.aligned()) {
+            rest = min(all, max(load.whole(), v0) - v0);
+            for (uint32_t v = tid; v < rest; v += 8 * kSlice) {
+                uint4 q[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) q[i] = __ldg(src + v + i * kSlice);
+                for (int i = 0; i < 8; ++i)
+                    if (v + i * kSlice < rest) q[i] = __ldg(src + v + i * kSlice);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) put(v + i * kSlice, q[i]);
+                for (int i = 0; i < 8; ++i)
+                    if (v + i * kSlice < rest) put(v + i * kSlice, q[i]);
+            }
+        } else {
+            rest = min(all, max(load.inner(), v0) - v0);
+            const uint32_t start = v0 == 0 ? 1 : 0;
+            if (start && tid == 0 && all) put(0, load(0));
+            for (uint32_t v = start + tid; v < rest; v += 4 * kSlice) {
+                uint4 lo[4], hi[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (v + i * kSlice < rest) {
+                        lo[i] = __ldg(src + v + i * kSlice);
+                        hi[i] = __ldg(src + v + i * kSlice + 1);
+                    }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (v + i * kSlice < rest) put(v + i * kSlice, load.shifted(lo[i], hi[i]));
+            }
+            rest = max(rest, start);
         }
-#pragma unroll 4
-        for (; v < easy; v += kSlice) put(v, __ldg(src + v));
-#pragma unroll 2
-        for (; v < all; v += kSlice) put(v, load(v0 + v));
+        for (uint32_t v = rest + tid; v < all; v += kSlice) put(v, load(v0 + v));
         for (int b = tid; b < kBins; b += kSlice) sh.hist[b] = 0;
         if (tid == 0) sh.listed = 0;
         top = vec_max<T>(m) + 0.0f;
@@ -534,16 +554,36 @@ sample_cluster_kernel(SampleArgs a, int shift, int ctas) {
     const int mode = k == 1 ? kFirst : floor_w >= 0.015625f ? kListing : by_count || by_mass || floor_w > 0.0f ? kCount : kRace;
     const float least_w = fmaxf(floor_w, 1.17549435e-38f);     // of the tokens that race (w > 0)
     uint4 race = JoinRace::none();
-    // the race of one vector's tokens: all their variates are requested before the first is used
-    auto enter = [&](const float (&x)[VEC], const float (&wx)[VEC], uint32_t i0) {
-        float e[VEC];
+    // The race of the tokens that weigh(vector, its first token, w[]) gives a w of least_w or more:
+    // the variates of 16 tokens per thread are requested before the first is used.
+    auto hold_race = [&](auto&& weigh) {
+        constexpr int U = 16 / VEC;
+        for (uint32_t v = tid; v < all; v += U * kSlice) {
+            float wx[U][VEC], e[U][VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) e[j] = wx[j] >= least_w ? __ldg(noise + i0 + j) : -1.0f;
+            for (int u = 0; u < U; ++u) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            if (!(e[j] >= 0.0f)) continue;
-            const uint32_t key = __float_as_uint(__fdividef(wx[j], e[j])) + 1;
-            if (key > race.x || (key == race.x && i0 + j < race.y)) { race.x = key; race.y = i0 + j; race.z = __float_as_uint(x[j]); }
+                for (int j = 0; j < VEC; ++j) wx[u][j] = 0.0f;
+                if (v + u * kSlice < all) weigh(slice[v + u * kSlice], (v0 + v + u * kSlice) * VEC, wx[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    e[u][j] = wx[u][j] >= least_w ? __ldg(noise + (v0 + v + u * kSlice) * VEC + j) : -1.0f;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    if (!(e[u][j] >= 0.0f)) continue;
+                    const uint32_t key = __float_as_uint(__fdividef(wx[u][j], e[u][j])) + 1;
+                    const uint32_t i = (v0 + v + u * kSlice) * VEC + j;
+                    if (key > race.x || (key == race.x && i < race.y)) {
+                        race.x = key;
+                        race.y = i;
+                        race.z = __float_as_uint(logit<T>(reinterpret_cast<const T*>(slice)[(v + u * kSlice) * VEC + j]));
+                    }
+                }
         }
     };
     auto list = [&](float x, uint32_t i) {
@@ -553,11 +593,10 @@ sample_cluster_kernel(SampleArgs a, int shift, int ctas) {
     };
     float z = 0.0f;
     uint32_t first = 0xFFFFFFFFu;
-    for (uint32_t v = tid, i0 = i_own; v < all; v += kSlice, i0 += kSlice * VEC) {
-        float x[VEC], wx[VEC];
-        unpack<T>(slice[v], x);
+    // a vector's exponents and w, and its part of Z
+    auto weigh_all = [&](const uint4& q, float (&x)[VEC], float2 (&y)[VEC / 2], float (&wx)[VEC]) {
+        unpack<T>(q, x);
         float2 zz = make_float2(0.0f, 0.0f);
-        float2 y[VEC / 2];
 #pragma unroll
         for (int j = 0; j < VEC; j += 2) {
             y[j / 2] = __fmul2_rn(__fadd2_rn(make_float2(x[j], x[j + 1]), make_float2(-top, -top)), make_float2(c, c));
@@ -566,6 +605,18 @@ sample_cluster_kernel(SampleArgs a, int shift, int ctas) {
             zz = __fadd2_rn(zz, make_float2(wx[j], wx[j + 1]));
         }
         z += zz.x + zz.y;
+    };
+    if (mode == kRace) {
+        hold_race([&](const uint4& q, uint32_t, float (&wx)[VEC]) {
+            float x[VEC];
+            float2 y[VEC / 2];
+            weigh_all(q, x, y, wx);
+        });
+    }
+    for (uint32_t v = tid, i0 = i_own; mode != kRace && v < all; v += kSlice, i0 += kSlice * VEC) {
+        float x[VEC], wx[VEC];
+        float2 y[VEC / 2];
+        weigh_all(slice[v], x, y, wx);
         if (mode == kListing) {
             float m = wx[0];
 #pragma unroll
@@ -581,8 +632,6 @@ sample_cluster_kernel(SampleArgs a, int shift, int ctas) {
                 const float t = (j & 1 ? y[j / 2].y : y[j / 2].x) * -kBinsPerOctave;
                 if (t < (float)kBins) atomicAdd(&sh.hist[(int)t], 1u);
             }
-        } else if (mode == kRace) {
-            enter(x, wx, i0);
         } else if (first == 0xFFFFFFFFu) {
 #pragma unroll
             for (int j = VEC - 1; j >= 0; --j)
@@ -657,17 +706,24 @@ sample_cluster_kernel(SampleArgs a, int shift, int ctas) {
         // race below goes on)
         const bool few = cut < kBins && sh.count[cut] <= (uint32_t)kList;
         if (few) cluster_barrier();     // the histograms have been read: CTA 0's list takes their place
-        for (uint32_t v = tid, i0 = i_own; v < all; v += kSlice, i0 += kSlice * VEC) {
-            const uint4 q = slice[v];
-            if (!(vec_max<T>(q) >= from)) continue;
-            float x[VEC], wx[VEC];
-            unpack<T>(q, x);
+        if (few) {
+            for (uint32_t v = tid, i0 = i_own; v < all; v += kSlice, i0 += kSlice * VEC) {
+                const uint4 q = slice[v];
+                if (!(vec_max<T>(q) >= from)) continue;
+                float x[VEC];
+                unpack<T>(q, x);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                wx[j] = x[j] >= from ? weight(x[j]) : 0.0f;
-                if (few && wx[j] >= least_w) list(x[j], i0 + j);
+                for (int j = 0; j < VEC; ++j)
+                    if (x[j] >= from && weight(x[j]) >= least_w) list(x[j], i0 + j);
             }
-            if (!few) enter(x, wx, i0);
+        } else {
+            hold_race([&](const uint4& q, uint32_t, float (&wx)[VEC]) {
+                if (!(vec_max<T>(q) >= from)) return;
+                float x[VEC];
+                unpack<T>(q, x);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) wx[j] = x[j] >= from ? weight(x[j]) : 0.0f;
+            });
         }
         if (few) {
             send();
@@ -698,15 +754,13 @@ sample_cluster_kernel(SampleArgs a, int shift, int ctas) {
         if (!have) {
             race = JoinRace::none();
             const float from = value_of(hi, shift);
-            for (uint32_t v = tid, i0 = i_own; v < all; v += kSlice, i0 += kSlice * VEC) {
-                const uint4 q = slice[v];
-                if (vec_max<T>(q) < from) continue;
-                float x[VEC], wx[VEC];
+            hold_race([&](const uint4& q, uint32_t i0, float (&wx)[VEC]) {
+                if (vec_max<T>(q) < from) return;
+                float x[VEC];
                 unpack<T>(q, x);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) wx[j] = position(x[j] + 0.0f, i0 + j, shift) < hi ? weight(x[j]) : 0.0f;
-                enter(x, wx, i0);
-            }
+            });
             won = cluster_join<JoinRace>(race, sh, turn, ctas, rank);
         }
         have = false;
