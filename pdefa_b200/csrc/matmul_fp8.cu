@@ -616,13 +616,31 @@ __device__ __forceinline__ void wide_store(const TcArgs& p, const CUtensorMap* t
             continue;
         }
         __syncwarp();
-        for (int i = lane; i < kWideChunks * kPer; i += 32) {
-            const int n = n0 + c + i, e = i % kPer;
-            if (n >= p.n) break;
-            const uint8_t* src = stage + i / kPer * kWideChunk;
-            for (int r = 0; r < rows && r < 32; ++r)
-                static_cast<T*>(p.out)[(int64_t)(row0 + r) * p.ldo + n] =
-                    reinterpret_cast<const T*>(src + r * 128 + (((e / kPiece) ^ r) & 7) * 16)[e % kPiece];
+        if (p.wide_out && n0 + c + kWideChunks * kPer <= p.n) {
+            // rows of a tile that the next expert shares: 16-byte pieces, two rows at a time
+            const int j = lane & 15;
+#pragma unroll
+            for (int i0 = 0; i0 < 16; i0 += 4) {
+                uint4 v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = (i0 + i) * 2 + (lane >> 4);
+                    v[i] = *reinterpret_cast<const uint4*>(stage + (j >> 3) * kWideChunk + r * 128 + ((j ^ r) & 7) * 16);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = (i0 + i) * 2 + (lane >> 4);
+                    if (r < rows) *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (int64_t)(row0 + r) * p.ldo + n0 + c + j * kPiece) = v[i];
+                }
+            }
+        } else {
+            // rows that do not start at multiples of 16 bytes (plan_matmul avoids them here), the last columns
+            for (int i = lane; i < kWideChunks * kPer && n0 + c + i < p.n; i += 32) {
+                const uint8_t* src = stage + i / kPer * kWideChunk + i % kPiece * sizeof(T);
+                for (int r = 0; r < 32 && r < rows; ++r)
+                    static_cast<T*>(p.out)[(int64_t)(row0 + r) * p.ldo + n0 + c + i] =
+                        *reinterpret_cast<const T*>(src + r * 128 + ((i % kPer / kPiece ^ r) & 7) * 16);
+            }
         }
         __syncwarp();
     }
@@ -987,20 +1005,23 @@ struct Plan { int wide, bt, split; };
 // 333 x 1201 x 2000: 32 over 1 9.8, 64 over 2 9.9, 128 over 4 11.0, wide 19; 512 x 4096 x 4096: 128
 // over 1 19.0, wide 22.2, 64 27.4; 800 x 4096 x 4096: wide 22.9, 128 33. Pairs where wide tiles
 // are more than one wave: 8192 x 8192 x 4096 267 against 277.
-Plan plan_matmul(const MatmulFp8Args& g, int64_t experts, int sms, int device) {
+Plan plan_matmul(const MatmulFp8Args& g, int64_t experts, int sms, int device, bool wide_out) {
     if (g.offsets) {
         // The experts' shares are on the GPU; what is known is the average. Tiles about twice
         // as wide as that hold most experts' rows at once. Measured (us, 64 experts, 2048 x 2048): 4 rows
         // each: 16 tokens 52.5, 32: 53.8, wide 55.7; 16 rows: 32: 56.1, 64: 63.1, wide 66.4, 16: 70.8; 32 rows: 64: 65.0,
         // wide 68.8, 128: 71.8; 64 rows: wide 71.3, 128: 76.1, 64: 103.
         const int64_t r = g.m / experts;
-        return r <= 6 ? Plan{0, 16, 1} : r <= 20 ? Plan{0, 32, 1} : r <= 48 ? Plan{0, 64, 1} : Plan{1, 128, 1};
+        // Output rows that do not start at multiples of 16 bytes cost a wide tile more than its
+        // products (8000 rows, 17 experts, 1041 x 912 bf16: wide 43, 128 tokens 37).
+        return r <= 6 ? Plan{0, 16, 1} : r <= 20 ? Plan{0, 32, 1} : r <= 64 && (r <= 48 || !wide_out) ? Plan{0, 64, 1}
+               : wide_out ? Plan{1, 128, 1} : Plan{0, 128, 1};
     }
     const int64_t nkb = (g.k + kBlock - 1) / kBlock, n_tiles = (g.n + kTileN - 1) / kTileN;
     auto waves = [&](int64_t tiles) { return (tiles + sms - 1) / sms; };
     const int64_t wide_tiles = (g.m + 127) / 128 * ((g.n + kWideN - 1) / kWideN);
     Plan best{wide_tiles > sms ? 2 : 1, 128, 1};
-    double least = (double)waves(wide_tiles) * (nkb * 0.5 + 1.2);
+    double least = (double)waves(wide_tiles) * (nkb * 0.5 + (wide_out ? 1.2 : 6.0));
     static const struct { int bt; double block, store, join; } kTiles[] = {
         {128, 0.33, 2.6, 5.2}, {64, 0.27, 2.1, 2.6}, {32, 0.26, 0.9, 1.7}, {16, 0.245, 0.1, 1.2}};
     for (const auto& c : kTiles) {
@@ -1073,9 +1094,9 @@ void launch_matmul_fp8(const MatmulFp8Args& g, cudaStream_t s) {
     p.err = device_error_word(device);
     p.wait_limit = 1000000000LL;
 
-    const Plan plan = plan_matmul(g, experts, sms, device);
-    const int wide = plan.wide, bt = wide ? 128 : plan.bt;
     p.wide_out = reinterpret_cast<uintptr_t>(g.out) % 16 == 0 && (g.m <= 1 || g.ldo * (g.out_dtype == ENGINE_F32 ? 4 : 2) % 16 == 0);
+    const Plan plan = plan_matmul(g, experts, sms, device, p.wide_out);
+    const int wide = plan.wide, bt = wide ? 128 : plan.bt;
     const int tokens = wide ? 128 * wide : bt;
     p.m_tiles = (int)((g.m + tokens - 1) / tokens);
 
