@@ -412,6 +412,35 @@ def test_sample_row_counts(rows, vocab):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("vocab", [3000, 33001])
+def test_sample_many_rows(vocab, dtype):
+    """More rows than run at once, with every setting and special rows among them."""
+    g = gen(vocab + 1)
+    rows = 20 * len(SETTINGS)
+    x, e = logits_of(g, rows, vocab, dtype), noise_of(g, rows, vocab)
+    inf = float("inf")
+    n = len(SETTINGS)
+    for i in range(n):                            # a special row of each kind under every setting
+        x[i] = -inf
+        x[n + i, 100:] = -inf
+        x[2 * n + i, [5, 2900]] = inf
+        x[3 * n + i, ::3] = float("nan")
+        x[4 * n + i] = torch.round(x[4 * n + i])
+        x[5 * n + i] = 2.5
+        e[6 * n + i] = float("nan")
+        x[7 * n + i] = torch.finfo(dtype).min
+        x[8 * n + i, 1500:] = torch.finfo(dtype).min
+        x[9 * n + i] *= 0.01                      # nearly even: long lists
+    cycle = [SETTINGS[i % n] for i in range(rows)]
+    tok, _ = check_sample(x, e, t=[s.get("t", 1.0) for s in cycle], k=[s.get("k", 0) for s in cycle],
+                          p=[s.get("p", 1.0) for s in cycle], m=[s.get("m", 0.0) for s in cycle])
+    assert (tok[:n] == -1).all()
+    again = pb.ops_sample(spaced(x, 3), spaced(e, 1))
+    want = pb.ops_sample(x, e)
+    assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
 @pytest.mark.parametrize("k,p", [(0, 1.0), (1, 1.0), (5, 1.0), (0, 0.5), (100, 0.3)])
 def test_sample_ties(dtype, k, p):
     """Equal logits are ordered by index: the filters cut inside a run of equals."""
