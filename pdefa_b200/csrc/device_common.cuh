@@ -189,4 +189,19 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
     return true;
 }
 
+// ---------------------------------------------------------------------------
+// Programmatic dependent launch. A kernel launched with the attribute may start while the
+// stream's previous kernel drains: grid_wait() returns once that one has finished and its
+// writes are visible, so every access to global memory comes after it. grid_trigger() lets
+// the next such kernel start once all CTAs of this one have called it.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+inline cudaLaunchAttribute dependent_launch() {
+    cudaLaunchAttribute a{};
+    a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    a.val.programmaticStreamSerializationAllowed = 1;
+    return a;
+}
+
 }  // namespace pb

@@ -240,6 +240,8 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
                      ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)S::kTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    grid_trigger();
+    grid_wait();                                             // what the stream wrote before is there
     if (warp == 2) {
         const int n = p.offsets ? build_table<BT>(p, table) : p.m_tiles;
         if (lane == 0) *tile_count = n;
@@ -694,6 +696,8 @@ matmul_fp8_wide_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_con
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
         }
     }
+    grid_trigger();
+    grid_wait();                                             // what the stream wrote before is there
     if (warp == 2) {
         const int n = p.offsets ? build_table<BT>(p, table) : p.m_tiles;
         if (lane == 0) *tile_count = n;
@@ -930,12 +934,13 @@ int tc_kernel(const TcArgs& args, int64_t grid, int split, const CUtensorMap* tm
     cfg.blockDim = dim3(S::kThreads);
     cfg.dynamicSmemBytes = fixed + (size_t)p.stages * (kABytes + S::kBBytes);
     cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)split;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute at[2];
+    at[0] = dependent_launch();
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)split;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = SPLIT ? 1 : 0;
+    cfg.numAttrs = SPLIT ? 2 : 1;
     if (!tmB) {
         int n = 0;
         PB_CUDA(cudaOccupancyMaxActiveClusters(&n, matmul_fp8_kernel<BT, SPLIT>, &cfg));
@@ -979,12 +984,13 @@ void launch_wide(const TcArgs& args, int64_t tiles, int sms, const CUtensorMap& 
     cfg.blockDim = dim3(kWideThreads);
     cfg.dynamicSmemBytes = fixed + (size_t)p.stages * stage;
     cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = CG;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute at[2];
+    at[0] = dependent_launch();
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = CG;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     PB_CUDA(cudaLaunchKernelEx(&cfg, matmul_fp8_wide_kernel<CG>, tmB, tmA, tmO, p));
 }
 

@@ -47,6 +47,8 @@ template <typename T, typename W>
 __global__ void __launch_bounds__(256)
 rms_norm_rows_kernel(RmsNormArgs a) {
     __shared__ float part[8];
+    grid_trigger();
+    grid_wait();
     const int64_t row = blockIdx.x;
     const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
     const T* res = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride : nullptr;
@@ -208,6 +210,8 @@ rms_norm_kernel(RmsNormArgs a) {
     __shared__ float part[32];
     __shared__ uint4 edge_h[ALIGNED ? 1 : N * 32 + 1];
     __shared__ uint4 edge_y[ALIGNED ? 1 : N * 32 + 1];
+    grid_trigger();
+    grid_wait();
     const int64_t row = blockIdx.x;
     const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
     const T* res = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride : nullptr;
@@ -346,6 +350,18 @@ rms_norm_kernel(RmsNormArgs a) {
     }
 }
 
+// A CTA per row.
+void launch_rows(void (*kernel)(RmsNormArgs), const RmsNormArgs& a, int threads, cudaStream_t s) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)a.rows);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.stream = s;
+    cudaLaunchAttribute at = dependent_launch();
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    PB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
+}
+
 template <typename T, typename W, int N, bool QUANT, bool ALIGNED>
 void launch_n(const RmsNormArgs& a, int64_t pieces, cudaStream_t s) {
     const int threads = (int)std::max<int64_t>(32, ((pieces + N - 1) / N + 31) / 32 * 32);
@@ -354,8 +370,8 @@ void launch_n(const RmsNormArgs& a, int64_t pieces, cudaStream_t s) {
     // 141 us against 173; 8192 x 4096: 37.9 against 40.9). Without one it is not (40000 x 2048
     // bf16: 53.3 against 50.4).
     const int64_t bytes = a.rows * a.cols * (int64_t)sizeof(T) * 3;
-    if (ALIGNED && a.residual && bytes > (int64_t(64) << 20)) rms_norm_kernel<T, W, N, QUANT, ALIGNED, ALIGNED><<<(unsigned)a.rows, threads, 0, s>>>(a);
-    else rms_norm_kernel<T, W, N, QUANT, ALIGNED, false><<<(unsigned)a.rows, threads, 0, s>>>(a);
+    const bool streams = ALIGNED && a.residual && bytes > (int64_t(64) << 20);
+    launch_rows(streams ? rms_norm_kernel<T, W, N, QUANT, ALIGNED, ALIGNED> : rms_norm_kernel<T, W, N, QUANT, ALIGNED, false>, a, threads, s);
 }
 
 // Pieces per thread: one for rows that all run at once (100 x 4096 bf16: 2.6 us, with two 3.0,
@@ -381,7 +397,7 @@ void launch_typed(const RmsNormArgs& a, cudaStream_t s) {
                          whole(a.h_out, a.h_stride, e, 16) && reinterpret_cast<uintptr_t>(a.weight) % 16 == 0 &&
                          (QUANT ? whole(a.y, a.y_stride, 1, kPiece<T>) : whole(a.y, a.y_stride, e, 16));
     if (aligned ? launch_pieces<T, W, QUANT, true>(a, s) : launch_pieces<T, W, QUANT, false>(a, s)) return;
-    rms_norm_rows_kernel<T, W><<<(unsigned)a.rows, 256, 0, s>>>(a);      // rows too long for the registers
+    launch_rows(rms_norm_rows_kernel<T, W>, a, 256, s);      // rows too long for the registers
 }
 
 template <typename T>
@@ -400,7 +416,6 @@ void launch_rms_norm(const RmsNormArgs& a, cudaStream_t s) {
         case ENGINE_BF16: launch_weights<__nv_bfloat16>(a, s); break;
         default: fail(ENGINE_ERR_INVALID_ARG, "rms_norm: dtype must be F32, F16 or BF16");
     }
-    PB_CUDA(cudaGetLastError());
 }
 
 }  // namespace pb

@@ -448,6 +448,8 @@ sample_cluster_kernel(SampleArgs a, int shift, int ctas) {
     const int tid = threadIdx.x;
     uint32_t rank;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    grid_trigger();
+    grid_wait();
     const int64_t row = blockIdx.x / ctas;
     const T* lg = static_cast<const T*>(a.logits) + row * a.logits_stride;
     const float* noise = a.noise + row * a.noise_stride;
@@ -834,12 +836,13 @@ bool launch_cluster(const SampleArgs& a, int shift, cudaStream_t s) {
     cfg.blockDim = dim3(kSlice);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)ctas;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute at[2];
+    at[0] = dependent_launch();
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)ctas;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     PB_CUDA(cudaLaunchKernelEx(&cfg, sample_cluster_kernel<T>, a, shift, ctas));
     return true;
 }
