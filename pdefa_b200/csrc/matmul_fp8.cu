@@ -6,16 +6,25 @@
 // a is [M, K] (rows are tokens), b is [N, K] (a weight as it is stored), or
 // [experts, N, K] with `offsets` giving each expert's range of rows of a.
 //
-// One warp-specialised tcgen05 kernel for all of it. A tile is 128 rows of the weight
-// (the M side of the instruction, its 128 TMEM lanes) times BT tokens (its N side, BT
-// TMEM columns), so a handful of tokens costs a narrow tile and not 128 padded rows.
+// Two warp-specialised tcgen05 kernels. The narrow one's tile is 128 rows of the weight
+// (the M side of the instruction, its 128 TMEM lanes) times 16 to 128 tokens (its N side,
+// TMEM columns), so a handful of tokens costs a narrow tile and not 128 padded rows; the
+// wide one's is 128 or 256 tokens (lanes) times 256 weight rows (columns).
+//
 // Scales change with every 128 k, so an accumulator cannot run through K on the tensor
 // core: each k-block (one 128-byte swizzled row per operand row, four instructions of
-// K = 32) goes into a fresh TMEM accumulator, and the epilogue warps add buffer * scale to
-// 32-bit sums in registers, while the tensor core fills the next buffer. The tile's
-// weight rows share one scale per k-block (tiles start at multiples of 128), the
-// tokens have one each; their products come from shared memory as one broadcast load
-// per four columns, and the sum is one packed fp32x2 multiply-add per two columns.
+// K = 32) goes into a fresh TMEM accumulator, and the epilogue warps add accumulator *
+// scale to 32-bit sums in registers while the tensor core fills the next. A weight tile of
+// 128 rows shares one scale per k-block (tiles start at multiples of 128), tokens have one
+// each. Narrow: the products of both scales come from shared memory as one broadcast load per
+// four columns. Wide: a lane is a token, so it has one scale per k-block. Either way the sum is
+// one packed fp32x2 multiply-add per two columns.
+//
+// What bounds them (B200). Few tokens: reading the weights, 64 rows over 64 experts of 2048 x
+// 2048 in 32 us, 5.3 TB/s; for one weight of 16 MB a launch and the pipeline's ends are most of
+// 6.2 us. Many tokens: TMEM, which the epilogue reads (128 KB per k-block and SM) beside the
+// tensor core; 8192 x 8192 x 4096 takes 265 us, 2076 TFLOP/s, at 990 cycles per k-block, where
+// products alone, without loads and epilogue, need 640 and the epilogue's reads 350.
 #include <algorithm>
 #include <atomic>
 #include <cuda.h>
@@ -477,7 +486,8 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
 // Many tokens: tiles of 128 * CG tokens (TMEM lanes, 128 per CTA) times 256 weight rows (TMEM
 // columns). CG = 2 is a pair of CTAs on one tile: each brings its own tokens and half of the
 // weight rows, and the tensor cores of both read both halves, so that a CTA moves 32 KB per
-// k-block instead of 48.
+// k-block instead of 48. (A product of 128 columns takes the tensor core as long as one of
+// 256, so finer accumulators that change hands earlier lose: 353 us against 277.)
 // ---------------------------------------------------------------------------
 constexpr int kWideN = 256;
 constexpr int kWideEpi = 8;
@@ -713,96 +723,96 @@ matmul_fp8_wide_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_con
     bool failed = false;
 
     if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideRegsLess));
-    if (warp == 0) {
-        if (lane == 0) {
-            RingPos rp;
-            int64_t it = 0;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideRegsLess));
+        if (warp == 0) {
+            if (lane == 0) {
+                RingPos rp;
+                int64_t it = 0;
+                for (int64_t t = t0; t < total && !failed; t += tstep) {
+                    const Tile tl = tile_of<BT, kWideN>(p, table, token_tiles, t);
+                    for (int kb = 0; kb < p.nkb; ++kb) {
+                        const int st = rp.slot;
+                        if (rp.wrapped && !mbar_wait_bounded(&empty[st], rp.phase ^ 1u, p.wait_limit)) {
+                            atomicExch(p.err, 31);
+                            failed = true;
+                            break;
+                        }
+                        rp.next(stages);
+                        ++it;
+                        if (rank == 0) mbar_expect_tx(&full[st], CG * (kA + kB));
+                        const uint32_t bar = CG == 2 ? mapa(smem_u32(&full[st]), 0) : smem_u32(&full[st]);
+                        wide_load_2d<CG>(base + (uint32_t)st * kA, &tmA, bar, kb * kBlock, tl.row0 + (int)rank * 128);
+                        wide_load_3d<CG>(ring_b + (uint32_t)st * kB, &tmB, bar, kb * kBlock, tl.n0 + (int)rank * 128, tl.expert);
+                    }
+                }
+                // the last load of every slot has landed before the CTA (or its pair) may exit
+                if (rank == 0)
+                    for (int64_t k = it > stages ? it - stages : 0; k < it; ++k)
+                        if (!mbar_wait_bounded(&full[k % stages], (uint32_t)((k / stages) & 1))) atomicExch(p.err, 32);
+            }
+            __syncwarp();
+        } else if (warp == 1) {
+            if (lane == 0 && rank == 0) {
+                const uint32_t idesc = (1u << 4) | ((uint32_t)(kWideN >> 3) << 17) | ((uint32_t)(BT >> 4) << 24);
+                RingPos rp, ap;
+                for (int64_t t = t0; t < total && !failed; t += tstep) {
+                    for (int kb = 0; kb < p.nkb; ++kb) {
+                        const int st = rp.slot, buf = ap.slot;
+                        if ((ap.wrapped && !mbar_wait_bounded(&tempty[buf], ap.phase ^ 1u, p.wait_limit)) ||
+                            !mbar_wait_bounded(&full[st], rp.phase, p.wait_limit)) {
+                            atomicExch(p.err, 33);
+                            failed = true;
+                            break;
+                        }
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        wide_mma<CG>(tmem + (uint32_t)(buf * kWideN), make_smem_desc(base + (uint32_t)st * kA, 128),
+                                     make_smem_desc(ring_b + (uint32_t)st * kB, 128), idesc);
+                        wide_commit<CG>(&empty[st]);
+                        wide_commit<CG>(&tfull[buf]);
+                        rp.next(stages);
+                        ap.next(2);
+                    }
+                }
+                wide_commit<CG>(mma_done);
+            }
+            __syncwarp();
+        } else if (warp == 2) {
+            // scales: chunk c holds sa[token] for kScaleChunk k-blocks, then sb of the two weight blocks
+            RingPos cp;
             for (int64_t t = t0; t < total && !failed; t += tstep) {
                 const Tile tl = tile_of<BT, kWideN>(p, table, token_tiles, t);
-                for (int kb = 0; kb < p.nkb; ++kb) {
-                    const int st = rp.slot;
-                    if (rp.wrapped && !mbar_wait_bounded(&empty[st], rp.phase ^ 1u, p.wait_limit)) {
-                        atomicExch(p.err, 31);
+                const int rows = tl.rows - (int)rank * 128;
+                const float* sa = p.sa + (int64_t)(tl.row0 + (int)rank * 128) * p.lda_scales;
+                const float* sb = p.sb + tl.expert * p.sb_expert + (tl.n0 / kBlock) * p.ldb_scales;
+                const bool second = tl.n0 + kBlock < p.n;
+                for (int kc = 0; kc < p.nkb && !failed; kc += kScaleChunk) {
+                    if (cp.wrapped && !warp_wait(&sempty[cp.slot], cp.phase ^ 1u, p.wait_limit)) {
+                        if (lane == 0) atomicExch(p.err, 34);
                         failed = true;
                         break;
                     }
-                    rp.next(stages);
-                    ++it;
-                    if (rank == 0) mbar_expect_tx(&full[st], CG * (kA + kB));
-                    const uint32_t bar = CG == 2 ? mapa(smem_u32(&full[st]), 0) : smem_u32(&full[st]);
-                    wide_load_2d<CG>(base + (uint32_t)st * kA, &tmA, bar, kb * kBlock, tl.row0 + (int)rank * 128);
-                    wide_load_3d<CG>(ring_b + (uint32_t)st * kB, &tmB, bar, kb * kBlock, tl.n0 + (int)rank * 128, tl.expert);
-                }
-            }
-            // the last load of every slot has landed before the CTA (or its pair) may exit
-            if (rank == 0)
-                for (int64_t k = it > stages ? it - stages : 0; k < it; ++k)
-                    if (!mbar_wait_bounded(&full[k % stages], (uint32_t)((k / stages) & 1))) atomicExch(p.err, 32);
-        }
-        __syncwarp();
-    } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
-            const uint32_t idesc = (1u << 4) | ((uint32_t)(kWideN >> 3) << 17) | ((uint32_t)(BT >> 4) << 24);
-            RingPos rp, ap;
-            for (int64_t t = t0; t < total && !failed; t += tstep) {
-                for (int kb = 0; kb < p.nkb; ++kb) {
-                    const int st = rp.slot, buf = ap.slot;
-                    if ((ap.wrapped && !mbar_wait_bounded(&tempty[buf], ap.phase ^ 1u, p.wait_limit)) ||
-                        !mbar_wait_bounded(&full[st], rp.phase, p.wait_limit)) {
-                        atomicExch(p.err, 33);
-                        failed = true;
-                        break;
+                    float* dst = scales + cp.slot * (kWideScales / 4);
+                    float v[4][kScaleChunk];
+    #pragma unroll
+                    for (int i = 0; i < 4; ++i)
+    #pragma unroll
+                        for (int j = 0; j < kScaleChunk; ++j)
+                            v[i][j] = i * 32 + lane < rows && kc + j < p.nkb ? __ldg(sa + (int64_t)(i * 32 + lane) * p.lda_scales + kc + j) : 0.0f;
+                    if (lane < 2 * kScaleChunk) {
+                        const int blk = lane / kScaleChunk, j = lane % kScaleChunk;
+                        dst[kScaleChunk * 128 + lane] = (blk == 0 || second) && kc + j < p.nkb ? __ldg(sb + blk * p.ldb_scales + kc + j) : 0.0f;
                     }
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    wide_mma<CG>(tmem + (uint32_t)(buf * kWideN), make_smem_desc(base + (uint32_t)st * kA, 128),
-                                 make_smem_desc(ring_b + (uint32_t)st * kB, 128), idesc);
-                    wide_commit<CG>(&empty[st]);
-                    wide_commit<CG>(&tfull[buf]);
-                    rp.next(stages);
-                    ap.next(2);
+    #pragma unroll
+                    for (int i = 0; i < 4; ++i)
+    #pragma unroll
+                        for (int j = 0; j < kScaleChunk; ++j) dst[j * 128 + i * 32 + lane] = v[i][j];
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sfull[cp.slot]);
+                    cp.next(2);
                 }
             }
-            wide_commit<CG>(mma_done);
+            __syncwarp();
         }
-        __syncwarp();
-    } else if (warp == 2) {
-        // scales: chunk c holds sa[token] for kScaleChunk k-blocks, then sb of the two weight blocks
-        RingPos cp;
-        for (int64_t t = t0; t < total && !failed; t += tstep) {
-            const Tile tl = tile_of<BT, kWideN>(p, table, token_tiles, t);
-            const int rows = tl.rows - (int)rank * 128;
-            const float* sa = p.sa + (int64_t)(tl.row0 + (int)rank * 128) * p.lda_scales;
-            const float* sb = p.sb + tl.expert * p.sb_expert + (tl.n0 / kBlock) * p.ldb_scales;
-            const bool second = tl.n0 + kBlock < p.n;
-            for (int kc = 0; kc < p.nkb && !failed; kc += kScaleChunk) {
-                if (cp.wrapped && !warp_wait(&sempty[cp.slot], cp.phase ^ 1u, p.wait_limit)) {
-                    if (lane == 0) atomicExch(p.err, 34);
-                    failed = true;
-                    break;
-                }
-                float* dst = scales + cp.slot * (kWideScales / 4);
-                float v[4][kScaleChunk];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < kScaleChunk; ++j)
-                        v[i][j] = i * 32 + lane < rows && kc + j < p.nkb ? __ldg(sa + (int64_t)(i * 32 + lane) * p.lda_scales + kc + j) : 0.0f;
-                if (lane < 2 * kScaleChunk) {
-                    const int blk = lane / kScaleChunk, j = lane % kScaleChunk;
-                    dst[kScaleChunk * 128 + lane] = (blk == 0 || second) && kc + j < p.nkb ? __ldg(sb + blk * p.ldb_scales + kc + j) : 0.0f;
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < kScaleChunk; ++j) dst[j * 128 + i * 32 + lane] = v[i][j];
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sfull[cp.slot]);
-                cp.next(2);
-            }
-        }
-        __syncwarp();
-    }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWideRegsMore));
         const int q = warp & 3, grp = (warp - 4) >> 2;       // TMEM lane quarter, group of columns
