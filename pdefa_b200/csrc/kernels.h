@@ -215,6 +215,7 @@ struct RmsNormArgs {
     int64_t rows = 0, cols = 0;
     int64_t x_stride = 0, residual_stride = 0, h_stride = 0, y_stride = 0, scales_stride = 0;
     float eps = 0.0f;
+    float inv_cols = 0.0f;             // 1 / cols, set by the launch
     int dtype = 0, weight_dtype = 0;   // weight: x's type or F32
     int quantize = 0;
 };

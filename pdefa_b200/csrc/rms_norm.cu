@@ -6,13 +6,14 @@
 //   8-bit: scale = max(max|y| over 128 columns, 1e-10) / 448, q = e4m3(y / scale)
 //
 // Bound by memory: the values are read once and written once, 16384 x 8192 bf16 with a
-// residual and an 8-bit output in 141 us (6.7 TB/s, 104% of a plain copy's rate on B200).
+// residual and an 8-bit output in 139 us (6.8 TB/s, 105% of a plain copy's rate on B200).
 //
 // The statistic and the scales come from the unrounded 32-bit sum. A NaN in a row
 // makes its whole output NaN (an infinity makes the statistic 0 and itself NaN).
 #include <algorithm>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
+#include <type_traits>
 
 #include "common.h"
 #include "device_common.cuh"
@@ -42,7 +43,13 @@ constexpr float kE4m3Max = 448.0f;
 constexpr float kTiny = 1e-10f;
 constexpr int kGroup = 128;
 
-// One CTA per row; every pass reads the row again (from L2 after the first).
+// 448 / m, within a few ulps of 32 bits: quotients by a scale are products by this, one fast
+// division per thread. (A quarter of both, since the fast division takes divisors to 2^126.)
+__device__ __forceinline__ float inverse_scale(float m) { return __fdividef(0.25f * kE4m3Max, 0.25f * m); }
+
+// One CTA per row; every pass reads the row again (from L2 after the first). For rows of more
+// than 4096 pieces, which the registers do not hold (1000 x 32776 bf16 with a residual and an
+// 8-bit output: 161 us; 1000 x 32760 in registers 51).
 template <typename T, typename W>
 __global__ void __launch_bounds__(256)
 rms_norm_rows_kernel(RmsNormArgs a) {
@@ -193,6 +200,79 @@ __device__ __forceinline__ V next_piece(const V& own, const V* edge, bool last_l
     return n;
 }
 
+// A piece with only elements lo .. hi - 1 kept.
+template <int BITS>
+__device__ __forceinline__ uint4 keep_range(const uint4& q, int lo, int hi) {
+    auto word = [&](uint32_t w, int k) {
+        const int from = min(max(lo * BITS - k * 32, 0), 32), to = min(max(hi * BITS - k * 32, 0), 32);
+        return w & __funnelshift_lc(~0u, 0u, to) & ~__funnelshift_lc(~0u, 0u, from);
+    };
+    return make_uint4(word(q.x, 0), word(q.y, 1), word(q.z, 2), word(q.w, 3));
+}
+// The first n elements (0 < n < 8 or 4) of an aligned piece, by words.
+template <typename E>
+__device__ __forceinline__ uint4 load_start(const E* p, int n) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(p);
+    const int words = n * (int)sizeof(E) / 4;
+    uint32_t q[4] = {0, 0, 0, 0}, last = 0;
+    if (sizeof(E) == 2 && (n & 1)) last = reinterpret_cast<const uint16_t*>(p)[n - 1];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) q[k] = k < words ? w[k] : k == words ? last : 0;
+    return make_uint4(q[0], q[1], q[2], q[3]);
+}
+// A piece of an array of n elements from anywhere in it, 0 outside: the two aligned pieces
+// around it, shifted.
+template <typename E>
+__device__ __forceinline__ uint4 load_anywhere(const E* array, int c, int n) {
+    constexpr int P = kPiece<E>;
+    const int off = (int)((reinterpret_cast<uintptr_t>(array) + (int64_t)c * (int)sizeof(E)) & 15);
+    const int first = c - off / (int)sizeof(E);
+    auto piece = [&](int at) {
+        if (at >= 0 && at + P <= n) return *reinterpret_cast<const uint4*>(array + at);
+        if (at >= n || at + P <= 0) return make_uint4(0, 0, 0, 0);
+        if (at >= 0) return load_start(array + at, n - at);
+        uint4 q = make_uint4(0, 0, 0, 0);           // the piece that holds an unaligned array's start
+        E* e = reinterpret_cast<E*>(&q);
+#pragma unroll
+        for (int j = 0; j < P; ++j)
+            if (at + j >= 0 && at + j < n) e[j] = array[at + j];
+        return q;
+    };
+    const uint4 lo = piece(first);
+    return off ? shift_pair(lo, piece(first + P), off >> 2, (off & 3) * 8) : lo;
+}
+// The bytes of a piece from `lo` on: halves of what is left, the smallest first where the piece
+// ends a row's lead (its end is aligned), the largest first where it starts a row's tail.
+__device__ __forceinline__ void put_bytes(uint8_t* at, uint4 q, int bytes, bool tail) {
+    auto drop = [&](int n) { q = shift_pair(q, make_uint4(0, 0, 0, 0), n >> 2, (n & 3) * 8); };
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int n = tail ? 8 >> k : 1 << k;
+        if (!(bytes & n)) continue;
+        if (n == 8) *reinterpret_cast<uint2*>(at) = make_uint2(q.x, q.y);
+        else if (n == 4) *reinterpret_cast<uint32_t*>(at) = q.x;
+        else if (n == 2) *reinterpret_cast<uint16_t*>(at) = (uint16_t)q.x;
+        else *at = (uint8_t)q.x;
+        at += n;
+        drop(n);
+    }
+}
+__device__ __forceinline__ uint4 widen(const uint4& q) { return q; }
+__device__ __forceinline__ uint4 widen(const uint2& q) { return make_uint4(q.x, q.y, 0, 0); }
+__device__ __forceinline__ uint4 widen(uint32_t q) { return make_uint4(q, 0, 0, 0); }
+// Stores the part of an aligned piece that lies in the row (of one piece at least).
+template <typename E, typename V>
+__device__ __forceinline__ void put_piece(E* row, int c, int cols, const V& v) {
+    constexpr int P = sizeof(V) / sizeof(E), S = sizeof(E);
+    if (c >= 0 && c + P <= cols) {
+        store_piece<false>(row + c, v);
+    } else if (c < 0) {
+        put_bytes(reinterpret_cast<uint8_t*>(row), shift_pair(widen(v), make_uint4(0, 0, 0, 0), -c * S >> 2, (-c * S & 3) * 8), (P + c) * S, false);
+    } else if (c < cols) {
+        put_bytes(reinterpret_cast<uint8_t*>(row + c), widen(v), (cols - c) * S, true);
+    }
+}
+
 template <int P> struct BytePiece;
 template <> struct BytePiece<8> { using type = uint2; };
 template <> struct BytePiece<4> { using type = uint32_t; };
@@ -201,7 +281,7 @@ template <> struct BytePiece<4> { using type = uint32_t; };
 // (i * threads + t) * kPiece. A group of 128 columns is 16 (or 32) neighbouring lanes.
 // !ALIGNED: rows of any alignment and length, read and written as aligned pieces that are
 // shifted into place. That takes twice the instructions, which then bound it (4000 x 8191 bf16
-// with a residual and an 8-bit output: 87 us, 2.7 TB/s; element by element 114 us).
+// with a residual and an 8-bit output: 84 us, 2.7 TB/s; element by element 114 us).
 template <typename T, typename W, int N, bool QUANT, bool ALIGNED, bool STREAM>
 __global__ void __launch_bounds__(1024)
 rms_norm_kernel(RmsNormArgs a) {
@@ -264,7 +344,7 @@ rms_norm_kernel(RmsNormArgs a) {
     sum = lane < warps ? part[lane] : 0.0f;
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    const float r = rsqrtf(sum / (float)cols + a.eps);
+    const float r = rsqrtf(sum * a.inv_cols + a.eps);
     uint4 out[N];               // the pieces of y
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -313,10 +393,8 @@ rms_norm_kernel(RmsNormArgs a) {
             }
 #pragma unroll
             for (int o = kGroup / P / 2; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(~0u, m, o));
-            if (c < cols && c % kGroup == 0) a.scales[row * a.scales_stride + c / kGroup] = m / kE4m3Max;
-            // the quotient by the scale as a product: one division per thread and not per value,
-            // within an ulp of 32 bits of it
-            const float inv = kE4m3Max / m;
+            if (c < cols && c % kGroup == 0) a.scales[row * a.scales_stride + c / kGroup] = m * (1.0f / kE4m3Max);
+            const float inv = inverse_scale(m);
             uint32_t b[2] = {0, 0};
 #pragma unroll
             for (int j = 0; j < P; j += 4) {
@@ -350,6 +428,167 @@ rms_norm_kernel(RmsNormArgs a) {
     }
 }
 
+// f(integral_constant of s), 0 <= s < P: a row's offset as a constant, so that which of a
+// piece's elements belong to which group costs no instructions.
+template <int P, typename F>
+__device__ __forceinline__ void by_offset(int s, F f) {
+    switch (s) {
+        case 0: f(std::integral_constant<int, 0>()); break;
+        case 1: f(std::integral_constant<int, 1>()); break;
+        case 2: f(std::integral_constant<int, 2>()); break;
+        case 3: f(std::integral_constant<int, 3>()); break;
+        case 4: f(std::integral_constant<int, P == 8 ? 4 : 0>()); break;
+        case 5: f(std::integral_constant<int, P == 8 ? 5 : 0>()); break;
+        case 6: f(std::integral_constant<int, P == 8 ? 6 : 0>()); break;
+        default: f(std::integral_constant<int, P == 8 ? 7 : 0>()); break;
+    }
+}
+
+// Rows of one kind of offset: x, the residual, h and y of a row all start at the same element of
+// an aligned piece, as those of contiguous tensors do whatever the number of columns. Pieces on
+// memory's own grid, which begins s columns before the row, are read and written as they are
+// and only the weights are shifted. A piece at the row's ends is read whole where the array goes
+// on beyond the row, and written by halves. The order in which the squares are added depends on s.
+// Bound by its instructions and its barriers, so registers are limited to what keeps three CTAs
+// of 544 threads on an SM (4000 x 8191 bf16, residual, 8-bit output: 60 us, the general kernel 84,
+// with one CTA on an SM 96; 4000 x 8190, 16-bit output: 51, general 84; 16000 x 2049, 8-bit: 51
+// against 57; 509 x 2050 f16: 2.6 against 3.0). Weights read early pay with one piece a thread only
+// (2.6 against 2.75; 55 against 51 with two).
+template <typename T, typename W, int N, bool QUANT>
+__global__ void __launch_bounds__(N == 2 ? 768 : 1024, N == 4 ? 1 : 2)
+rms_norm_alike_kernel(RmsNormArgs a) {
+    constexpr int P = kPiece<T>, PW = kPiece<W>, H = kGroup / P;
+    using Q = typename BytePiece<P>::type;
+    __shared__ float part[32];
+    // Largest |y| of a group without its end, and of that end, which is the first s elements of
+    // the next group's first piece.
+    __shared__ float top[QUANT ? N * 1024 / H : 1], low[QUANT ? N * 1024 / H : 1], inv[QUANT ? N * 1024 / H : 1];
+    grid_trigger();
+    grid_wait();
+    const int64_t row = blockIdx.x;
+    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+    const T* res = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride : nullptr;
+    const W* w = static_cast<const W*>(a.weight);
+    T* h_out = a.h_out ? static_cast<T*>(a.h_out) + row * a.h_stride : nullptr;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int threads = blockDim.x, warps = threads >> 5, cols = (int)a.cols;
+    const int s = (int)(reinterpret_cast<uintptr_t>(x) / sizeof(T) % P);
+    const bool x_front = row * a.x_stride >= P, x_back = (a.rows - 1 - row) * a.x_stride >= P;
+    const bool r_front = row * a.residual_stride >= P, r_back = (a.rows - 1 - row) * a.residual_stride >= P;
+    uint4 qx[N], qr[N];
+    float v[N][P];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int c = (i * threads + (int)threadIdx.x) * P - s;
+        qx[i] = qr[i] = make_uint4(0, 0, 0, 0);
+        // whole pieces, those at the row's ends too where the array goes on beyond the row
+        const bool x_whole = (c >= 0 || x_front) && (c + P <= cols || x_back);
+        const bool r_whole = (c >= 0 || r_front) && (c + P <= cols || r_back);
+        if (c < cols) {
+            if (x_whole) qx[i] = load_piece<false>(x + c);
+            if (res && r_whole) qr[i] = load_piece<false>(res + c);
+            if (!x_whole) qx[i] = load_anywhere(x, c, cols);
+            if (res && !r_whole) qr[i] = load_anywhere(res, c, cols);
+        }
+    }
+    uint4 wq[P / PW];                       // one piece's weights are read before the sum is known
+    if (N == 1) {
+#pragma unroll
+        for (int j = 0; j < P / PW; ++j) wq[j] = load_anywhere(w, (int)threadIdx.x * P - s + j * PW, cols);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int c = (i * threads + (int)threadIdx.x) * P - s;
+        if (c < 0 || c + P > cols) {
+            qx[i] = keep_range<8 * sizeof(T)>(qx[i], -c, cols - c);
+            qr[i] = keep_range<8 * sizeof(T)>(qr[i], -c, cols - c);
+        }
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        unpack<T>(qx[i], v[i]);
+        if (res) {
+            float r[P];
+            unpack<T>(qr[i], r);
+#pragma unroll
+            for (int j = 0; j < P; ++j) v[i][j] += r[j];
+        }
+#pragma unroll
+        for (int j = 0; j < P; ++j) sum = fmaf(v[i][j], v[i][j], sum);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    if (lane == 0) part[warp] = sum;
+    __syncthreads();
+    sum = lane < warps ? part[lane] : 0.0f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    const float r = rsqrtf(sum * a.inv_cols + a.eps);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int u = i * threads + (int)threadIdx.x, c = u * P - s;
+        if (h_out) put_piece(h_out, c, cols, pack<T>(v[i]));
+#pragma unroll
+        for (int j = 0; j < P; j += PW) {
+            float f[PW];
+            unpack<W>(N == 1 ? wq[j / PW] : load_anywhere(w, c + j, cols), f);
+#pragma unroll
+            for (int t = 0; t < PW; ++t) v[i][j + t] = v[i][j + t] * r * f[t];
+        }
+        if (!QUANT) {
+            put_piece(static_cast<T*>(a.y) + row * a.y_stride, c, cols, pack<T>(v[i]));
+        } else {
+            float m = kTiny, end = kTiny;
+            by_offset<P>(s, [&](auto S) {
+#pragma unroll
+                for (int j = 0; j < P; ++j) {
+                    if (j < S.value) end = max_nan(end, fabsf(v[i][j]));
+                    else m = max_nan(m, fabsf(v[i][j]));
+                }
+            });
+            if (lane % H) m = max_nan(m, end);
+#pragma unroll
+            for (int o = H / 2; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(~0u, m, o));
+            if (lane % H == 0) {
+                top[u / H] = m;
+                low[u / H] = end;
+            }
+        }
+    }
+    if (!QUANT) return;
+    __syncthreads();
+    const int groups = N * threads / H;             // fewer than threads
+    if ((int)threadIdx.x < groups && (int)threadIdx.x * kGroup < cols) {
+        const int g = threadIdx.x;
+        const float m = g + 1 < groups ? max_nan(top[g], low[g + 1]) : top[g];
+        a.scales[row * a.scales_stride + g] = m * (1.0f / kE4m3Max);
+        inv[g] = inverse_scale(m);      
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int u = i * threads + (int)threadIdx.x, c = u * P - s;
+        if (c >= cols) continue;
+        const int own = min(u / H, (cols - 1) / kGroup);        // the last piece may only end a group
+        const float f_own = inv[own], f_end = inv[lane % H || u == 0 ? own : u / H - 1];
+        uint32_t b[2] = {0, 0};
+        by_offset<P>(s, [&](auto S) {
+#pragma unroll
+            for (int j = 0; j < P; j += 4) {
+                float f[4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) f[t] = v[i][j + t] * (j + t < S.value ? f_end : f_own);
+                const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3);
+                const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[2], f[3]), __NV_SATFINITE, __NV_E4M3);
+                b[j / 4] = lo | hi << 16;
+            }
+        });
+        const uint2 q = make_uint2(b[0], b[1]);
+        put_piece(static_cast<uint8_t*>(a.y) + row * a.y_stride, c, cols, *reinterpret_cast<const Q*>(&q));
+    }
+}
+
 // A CTA per row.
 void launch_rows(void (*kernel)(RmsNormArgs), const RmsNormArgs& a, int threads, cudaStream_t s) {
     cudaLaunchConfig_t cfg{};
@@ -362,41 +601,56 @@ void launch_rows(void (*kernel)(RmsNormArgs), const RmsNormArgs& a, int threads,
     PB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
 }
 
-template <typename T, typename W, int N, bool QUANT, bool ALIGNED>
+enum class Rows { kWhole, kAlike, kAny };       // whole aligned pieces, one kind of offset, any
+
+template <typename T, typename W, int N, bool QUANT, Rows ROWS>
 void launch_n(const RmsNormArgs& a, int64_t pieces, cudaStream_t s) {
     const int threads = (int)std::max<int64_t>(32, ((pieces + N - 1) / N + 31) / 32 * 32);
-    // With a residual, four arrays go through the L2 cache; beyond half of its 126 MB they only
-    // push each other out, and passing them through is faster (16384 x 8192 bf16, 8-bit output:
-    // 141 us against 173; 8192 x 4096: 37.9 against 40.9). Without one it is not (40000 x 2048
-    // bf16: 53.3 against 50.4).
-    const int64_t bytes = a.rows * a.cols * (int64_t)sizeof(T) * 3;
-    const bool streams = ALIGNED && a.residual && bytes > (int64_t(64) << 20);
-    launch_rows(streams ? rms_norm_kernel<T, W, N, QUANT, ALIGNED, ALIGNED> : rms_norm_kernel<T, W, N, QUANT, ALIGNED, false>, a, threads, s);
+    if constexpr (ROWS == Rows::kAny) {
+        launch_rows(rms_norm_kernel<T, W, N, QUANT, false, false>, a, threads, s);
+    } else if constexpr (ROWS == Rows::kAlike) {
+        launch_rows(rms_norm_alike_kernel<T, W, N, QUANT>, a, threads, s);
+    } else {
+        // With a residual, four arrays go through the L2 cache; beyond half of its 126 MB they only
+        // push each other out, and passing them through is faster (16384 x 8192 bf16, 8-bit output:
+        // 139 us against 173; 8192 x 4096: 37.9 against 40.9). Without one it is not (40000 x 2048
+        // bf16: 53.3 against 50.4), nor where rows share their ends' lines (8000 x 4001: 49.1
+        // against 47.5).
+        const bool streams = a.residual && a.rows * a.cols * (int64_t)sizeof(T) * 3 > (int64_t(64) << 20);
+        launch_rows(streams ? rms_norm_kernel<T, W, N, QUANT, true, true> : rms_norm_kernel<T, W, N, QUANT, true, false>, a, threads, s);
+    }
 }
 
-// Pieces per thread: one for rows that all run at once (100 x 4096 bf16: 2.6 us, with two 3.0,
-// with four 3.9), two for more rows (16384 x 8192: 141 us, one 182, four 142), four for rows
-// that two do not hold.
-template <typename T, typename W, bool QUANT, bool ALIGNED>
+// Pieces per thread: one where all rows run at once (550 x 4096 bf16, residual, 8-bit: 3.5 us, with
+// two 4.5; 509 x 2050 f16: 2.6 and 4.1), two for more rows (16384 x 8192: 139 us, one 182, four 142;
+// 500 x 6001: 6.4, one 8.2), four for rows that two do not hold.
+template <typename T, typename W, bool QUANT, Rows ROWS>
 bool launch_pieces(const RmsNormArgs& a, cudaStream_t s) {
-    const int64_t pieces = (a.cols + kPiece<T> - 1) / kPiece<T>;
+    const int64_t ends = ROWS == Rows::kAlike ? kPiece<T> - 1 : 0;      // columns before the row in its first piece
+    const int64_t pieces = (a.cols + ends + kPiece<T> - 1) / kPiece<T>;
     if (pieces > 4 * 1024) return false;
-    if (pieces > 2 * 1024) launch_n<T, W, 4, QUANT, ALIGNED>(a, pieces, s);
-    else if (pieces > 1024 || (a.rows > 296 && pieces > 32)) launch_n<T, W, 2, QUANT, ALIGNED>(a, pieces, s);
-    else launch_n<T, W, 1, QUANT, ALIGNED>(a, pieces, s);
+    const int64_t most = ROWS == Rows::kAlike ? 768 : 1024;     // threads, with two pieces each
+    const bool at_once = a.rows * ((pieces + 31) / 32 * 32) <= 148 * 2048;
+    if (pieces > 2 * most) launch_n<T, W, 4, QUANT, ROWS>(a, pieces, s);
+    else if (pieces > 1024 || (!at_once && pieces > 32)) launch_n<T, W, 2, QUANT, ROWS>(a, pieces, s);
+    else launch_n<T, W, 1, QUANT, ROWS>(a, pieces, s);
     return true;
 }
 
 template <typename T, typename W, bool QUANT>
 void launch_typed(const RmsNormArgs& a, cudaStream_t s) {
-    auto whole = [&](const void* p, int64_t stride, int64_t bytes, int64_t piece) {
-        return !p || (reinterpret_cast<uintptr_t>(p) % piece == 0 && (a.rows <= 1 || stride * bytes % piece == 0));
+    // Do an array's rows start at the same element of an aligned piece as x's?
+    auto alike = [&](const void* p, int64_t stride, int64_t bytes) {
+        const int64_t at = (int64_t)(reinterpret_cast<uintptr_t>(p) / bytes) - (int64_t)(reinterpret_cast<uintptr_t>(a.x) / sizeof(T));
+        return !p || (at % kPiece<T> == 0 && (a.rows <= 1 || (stride - a.x_stride) % kPiece<T> == 0));
     };
     const int64_t e = sizeof(T);
-    const bool aligned = a.cols % kPiece<T> == 0 && whole(a.x, a.x_stride, e, 16) && whole(a.residual, a.residual_stride, e, 16) &&
-                         whole(a.h_out, a.h_stride, e, 16) && reinterpret_cast<uintptr_t>(a.weight) % 16 == 0 &&
-                         (QUANT ? whole(a.y, a.y_stride, 1, kPiece<T>) : whole(a.y, a.y_stride, e, 16));
-    if (aligned ? launch_pieces<T, W, QUANT, true>(a, s) : launch_pieces<T, W, QUANT, false>(a, s)) return;
+    const bool same = alike(a.residual, a.residual_stride, e) && alike(a.h_out, a.h_stride, e) && alike(a.y, a.y_stride, QUANT ? 1 : e);
+    const bool whole = same && a.cols % kPiece<T> == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 &&
+                       (a.rows <= 1 || a.x_stride % kPiece<T> == 0) && reinterpret_cast<uintptr_t>(a.weight) % 16 == 0;
+    if (whole && launch_pieces<T, W, QUANT, Rows::kWhole>(a, s)) return;
+    if (!whole && same && a.cols >= 2 * kPiece<T> && launch_pieces<T, W, QUANT, Rows::kAlike>(a, s)) return;
+    if (!whole && launch_pieces<T, W, QUANT, Rows::kAny>(a, s)) return;
     launch_rows(rms_norm_rows_kernel<T, W>, a, 256, s);      // rows too long for the registers
 }
 
@@ -408,8 +662,10 @@ void launch_weights(const RmsNormArgs& a, cudaStream_t s) {
 
 }  // namespace
 
-void launch_rms_norm(const RmsNormArgs& a, cudaStream_t s) {
-    if (a.rows == 0 || a.cols == 0) return;
+void launch_rms_norm(const RmsNormArgs& args, cudaStream_t s) {
+    if (args.rows == 0 || args.cols == 0) return;
+    RmsNormArgs a = args;
+    a.inv_cols = 1.0f / (float)a.cols;
     switch (a.dtype) {
         case ENGINE_F32: launch_weights<float>(a, s); break;
         case ENGINE_F16: launch_weights<__half>(a, s); break;

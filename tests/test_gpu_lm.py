@@ -95,6 +95,40 @@ def test_norm(rows, cols, dtype, residual, gap):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids)
+@pytest.mark.parametrize("rows,cols", [(9, 17), (40, 131), (13, 1031), (1100, 1153), (700, 3001), (9, 8191), (11, 13001),
+                                       (7, 16383), (3, 32761)])
+def test_norm_rows_of_every_offset(rows, cols, dtype):
+    """Contiguous rows of odd lengths start at every offset within 16 bytes; what lies beside a row stays out of it."""
+    g = gen(rows + cols)
+    x, res = (randn(g, rows, cols) * 3).to(dtype), randn(g, rows, cols).to(dtype)
+    x[1::3] = float("nan")
+    w = (1 + 0.3 * randn(g, cols)).to(dtype)
+    fine = [i for i in range(rows) if i % 3 != 1]
+    tol = (cols / 128 + 32) * U
+    nb = -(-cols // 128)
+    for r in (None, res):
+        y64, h64 = norm_ref(x[fine], w, None if r is None else r[fine], 1e-5)
+        got = pb.ops_rms_norm(x, w, residual=r, eps=1e-5)
+        y, h = got if r is not None else (got, None)
+        assert ((y[fine].double() - y64).abs() <= (tol + V[dtype]) * y64.abs() * 1.0001 + LEAST[dtype]).all()
+        assert y[1::3].isnan().all()
+        got = pb.ops_rms_norm_fp8(x, w, residual=r, eps=1e-5)
+        pad = torch.nn.functional.pad(y64, (0, nb * 128 - cols)).view(len(fine), nb, 128)
+        s64 = pad.abs().amax(-1).clamp(min=1e-10) / 448
+        assert ((got[1][fine].double() - s64).abs() <= (tol + 4 * U) * s64).all()
+        assert got[1][1::3].isnan().all()
+        unit = (pad / s64[..., None]).view(len(fine), -1)[:, :cols]
+        far = (got[0][fine].double() - unit).abs()
+        assert (far <= torch.clamp(unit.abs() * 2.0 ** -4, min=2.0 ** -10) * 1.001 + 448 * (tol + 8 * U)).all()
+        if r is not None:
+            want = (x.float() + res.float()).to(dtype)
+            assert torch.equal(h[fine], want[fine]) and h[1::3].isnan().all()
+            assert torch.equal(got[2][fine], want[fine])
+    one = pb.ops_rms_norm(x[:1], w)
+    assert torch.equal(pb.ops_rms_norm(x[:1].expand(5, cols), w), one.expand(5, cols))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids)
 def test_norm_special_rows(dtype):
     g = gen(5)
     cols = 384
