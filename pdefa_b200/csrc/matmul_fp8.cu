@@ -183,6 +183,16 @@ __device__ __forceinline__ void store_out(void* out, int dtype, int64_t i, float
 }
 
 // Four columns of a row, n a multiple of 4.
+__device__ __forceinline__ void convert(float* d, float v) { *d = v; }
+__device__ __forceinline__ void convert(__half* d, float v) { *d = __float2half_rn(v); }
+__device__ __forceinline__ void convert(__nv_bfloat16* d, float v) { *d = __float2bfloat16_rn(v); }
+// One weight row's values of up to N tokens; the lanes of a warp hold neighbouring ones.
+template <int N, typename T>
+__device__ __forceinline__ void store_column(T* d, int64_t ldo, int most, const float* v) {
+#pragma unroll
+    for (int i = 0; i < N; ++i, d += ldo)
+        if (i < most) convert(d, v[i]);
+}
 __device__ __forceinline__ void store_out4(const TcArgs& p, int row, int n, float4 v) {
     const int64_t at = (int64_t)row * p.ldo + n;
     if (p.wide_out && n + 4 <= p.n) {
@@ -423,11 +433,11 @@ matmul_fp8_kernel(const __grid_constant__ CUtensorMap tmB, const __grid_constant
             }
             if (SPLIT || failed) continue;
             const int n = mine.n0 + q * 32 + lane;
-            if (n < p.n) {
-#pragma unroll
-                for (int i = 0; i < S::kCols; ++i)
-                    if (c0 + i < mine.rows) store_out(p.out, p.out_dtype, (int64_t)(mine.row0 + c0 + i) * p.ldo + n, acc[i]);
-            }
+            const int most = n < p.n ? mine.rows - c0 : 0;
+            const int64_t at = (int64_t)(mine.row0 + c0) * p.ldo + n;
+            if (p.out_dtype == ENGINE_BF16) store_column<S::kCols>(static_cast<__nv_bfloat16*>(p.out) + at, p.ldo, most, acc);
+            else if (p.out_dtype == ENGINE_F16) store_column<S::kCols>(static_cast<__half*>(p.out) + at, p.ldo, most, acc);
+            else store_column<S::kCols>(static_cast<float*>(p.out) + at, p.ldo, most, acc);
         }
         if (!SPLIT && p.offsets) {
             // rows before the first and after the last expert's
@@ -646,12 +656,23 @@ __device__ __forceinline__ void wide_store(const TcArgs& p, const CUtensorMap* t
                 }
             }
         } else {
-            // rows that do not start at multiples of 16 bytes (plan_matmul avoids them here), the last columns
-            for (int i = lane; i < kWideChunks * kPer && n0 + c + i < p.n; i += 32) {
+            // rows that do not start at multiples of 16 bytes, the last columns: a column per
+            // lane, eight rows at a time (row by row a tile took 6 us and not 4.5)
+#pragma unroll
+            for (int i0 = 0; i0 < kWideChunks * kPer; i0 += 32) {
+                const int i = i0 + lane;
                 const uint8_t* src = stage + i / kPer * kWideChunk + i % kPiece * sizeof(T);
-                for (int r = 0; r < 32 && r < rows; ++r)
-                    static_cast<T*>(p.out)[(int64_t)(row0 + r) * p.ldo + n0 + c + i] =
-                        *reinterpret_cast<const T*>(src + r * 128 + ((i % kPer / kPiece ^ r) & 7) * 16);
+                T* dst = static_cast<T*>(p.out) + (int64_t)row0 * p.ldo + n0 + c + i;
+                const int most = n0 + c + i < p.n ? rows : 0;
+#pragma unroll
+                for (int r0 = 0; r0 < 32; r0 += 8) {
+                    T v[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[k] = *reinterpret_cast<const T*>(src + (r0 + k) * 128 + ((i % kPer / kPiece ^ k) & 7) * 16);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (r0 + k < most) dst[(r0 + k) * p.ldo] = v[k];
+                }
             }
         }
         __syncwarp();
@@ -1016,30 +1037,34 @@ struct Plan { int wide, bt, split; };
 // them the busiest CTA gets. With one weight all shapes are known: of every tile the time of
 // the busiest CTA is waves * (k-blocks * time of one + time to store the tile), or with a split
 // the k-blocks' and the joining's, and the least wins. The times (us) are fits to a sweep on
-// a B200, which they meet within 10%. Measured, m x n x k: 16 x 4096 x 4096: 16 tokens over 4
-// CTAs 7.5, over 2 9.1, over 1 12.3; 64 x 4096 x 4096: 64 over 4 8.9, 32 over 2 10.2, 16 over 1 12.6;
-// 333 x 1201 x 2000: 32 over 1 9.8, 64 over 2 9.9, 128 over 4 11.0, wide 19; 512 x 4096 x 4096: 128
-// over 1 19.0, wide 22.2, 64 27.4; 800 x 4096 x 4096: wide 22.9, 128 33. Pairs where wide tiles
-// are more than one wave: 8192 x 8192 x 4096 267 against 277.
+// a B200, which they meet within 10% or so; the plan's time is within 9% of the best one's for 469
+// shapes of a sweep (mean 0.5%). Measured, m x n x k, bf16 out: 16 x 4096 x 4096: 16 tokens over 4 CTAs
+// 7.5, over 2 9.1, over 1 12.3; 333 x 2048 x 272: 64: 5.3, 32: 5.8, 128: 6.3, wide 6.9; 2000 x 4096 x 1024:
+// wide 15.3, 128: 20.9, 64: 23.3. Rows that do not start at multiples of 16 bytes: 2000 x 4097 x 1024: wide
+// 19.2, 128: 22.0; f32 4000 x 4097 x 1024: 128: 43.6, 64: 46.4, wide 51.4. Pairs where wide tiles are
+// more than one wave: 8192 x 8192 x 4096 267 against 277.
 Plan plan_matmul(const MatmulFp8Args& g, int64_t experts, int sms, int device, bool wide_out) {
     if (g.offsets) {
-        // The experts' shares are on the GPU; what is known is the average. Tiles about twice
-        // as wide as that hold most experts' rows at once. Measured (us, 64 experts, 2048 x 2048): 4 rows
-        // each: 16 tokens 52.5, 32: 53.8, wide 55.7; 16 rows: 32: 56.1, 64: 63.1, wide 66.4, 16: 70.8; 32 rows: 64: 65.0,
-        // wide 68.8, 128: 71.8; 64 rows: wide 71.3, 128: 76.1, 64: 103.
+        // The experts' shares are on the GPU; what is known is the average. Measured, as the mean over
+        // 15 shapes of the time over the best tile's (8 to 64 experts, even and uneven, 1024 to 2048 wide,
+        // 512 to 2048 long, 16-bit output): 8 rows each: 16 tokens 1.00, 32: 1.04; 16 rows: 32: 1.01,
+        // 64: 1.14, 16: 1.15; 32 rows: 64: 1.01, 32: 1.09, wide 1.22; 48 rows: 64: 1.02, wide 1.17; 64 rows:
+        // wide 1.08, 64: 1.13, 128: 1.15; 256 rows: wide 1.00, 128: 1.24. Output rows that do not start at
+        // multiples of 16 bytes cost a wide tile 2.3 more, and 6.5 in 32 bits: 64 rows: 64: 1.04, 128: 1.09,
+        // wide 1.18; 96 rows: 128: 1.08, wide 1.14; 128 rows: wide 1.05, 128: 1.08; 512 rows: wide 1.01,
+        // 128: 1.09; in 32 bits 512 rows: 128: 1.00, wide 1.26.
         const int64_t r = g.m / experts;
-        // Output rows that do not start at multiples of 16 bytes cost a wide tile more than its
-        // products (8000 rows, 17 experts, 1041 x 912 bf16: wide 43, 128 tokens 37).
-        return r <= 6 ? Plan{0, 16, 1} : r <= 20 ? Plan{0, 32, 1} : r <= 64 && (r <= 48 || !wide_out) ? Plan{0, 64, 1}
-               : wide_out ? Plan{1, 128, 1} : Plan{0, 128, 1};
+        if (r <= 48) return Plan{0, r <= 8 ? 16 : r <= 20 ? 32 : 64, 1};
+        if (wide_out || (r >= 112 && g.out_dtype != ENGINE_F32)) return Plan{1, 128, 1};
+        return Plan{0, r <= 80 ? 64 : 128, 1};
     }
     const int64_t nkb = (g.k + kBlock - 1) / kBlock, n_tiles = (g.n + kTileN - 1) / kTileN;
     auto waves = [&](int64_t tiles) { return (tiles + sms - 1) / sms; };
     const int64_t wide_tiles = (g.m + 127) / 128 * ((g.n + kWideN - 1) / kWideN);
     Plan best{wide_tiles > sms ? 2 : 1, 128, 1};
-    double least = (double)waves(wide_tiles) * (nkb * 0.5 + (wide_out ? 1.2 : 6.0));
+    double least = (double)waves(wide_tiles) * (nkb * 0.505 + (wide_out ? 2.2 : g.out_dtype == ENGINE_F32 ? 8.7 : 4.5));
     static const struct { int bt; double block, store, join; } kTiles[] = {
-        {128, 0.33, 2.6, 5.2}, {64, 0.27, 2.1, 2.6}, {32, 0.26, 0.9, 1.7}, {16, 0.245, 0.1, 1.2}};
+        {128, 0.345, 2.3, 5.7}, {64, 0.264, 1.05, 3.1}, {32, 0.24, 0.65, 2.2}, {16, 0.237, 0.55, 1.7}};
     for (const auto& c : kTiles) {
         const int64_t tiles = (g.m + c.bt - 1) / c.bt * n_tiles;
         for (int split = 1; split <= 8; split *= 2) {
