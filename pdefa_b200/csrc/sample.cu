@@ -19,6 +19,12 @@
 // winner. The same counting pass also tests the midpoint between the last position
 // known to be kept and `hi`, so rounds are bounded by the bits of a position whatever
 // the variates are; with random ones there are one or two.
+//
+// A row is read once into the shared memory of a cluster. What bounds it is not that read but
+// the phases after it, each a barrier and an exchange over the cluster's CTAs (1 to 1.3 us):
+// 256 x 131072 bf16 with top-k, top-p and min-p 50 us (1.3 TB/s; the read alone 10), one row of
+// 32000 6.4 us. So rows are spread over CTAs to have all of them in flight at once, candidates are
+// counted before they are listed, and what one CTA can finish alone is sent to one.
 #include <algorithm>
 #include <cuda_fp16.h>
 
@@ -100,6 +106,8 @@ __device__ __forceinline__ Race warp_race(Race r) {
     return r;
 }
 
+// A CTA per row that reads the row again in every pass, for rows that a cluster's shared memory
+// does not hold (8 slices of 200 KB; 16 x 409700 f32: 579 us, 16 x 409600 by clusters 31).
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 sample_rows_kernel(SampleArgs a, int shift) {
@@ -817,12 +825,21 @@ bool launch_cluster(const SampleArgs& a, int shift, cudaStream_t s) {
     const int64_t bytes = a.vocab * (int64_t)sizeof(T);
     constexpr int64_t kMost = 200 * 1024;      // of a slice
     if (bytes / kMostCtas > kMost) return false;
-    // As many CTAs per row as leave every row's cluster resident at once (two CTAs an SM), but
-    // enough for slices of 64 KB. Measured (us, bf16 unless said): 1 row of 32000: 8 CTAs 6.1, 2 CTAs 7.2;
-    // 33 of 50257 (f32): 8: 16.0, 4: 18.2; 64 of 131072: 4: 15.9, 8: 21.3, 2: 17.0; 128 of 32000 (f32):
-    // 2: 22.0, 4: 24.3; 256 of 131072: 4: 48.6, 2: 54.7, 8: 66.9.
-    const int64_t fit = 2 * 148 / a.rows, need = (bytes + 65535) / 65536;
-    const int ctas = (int)std::min<int64_t>(kMostCtas, std::max(fit, need));
+    // CTAs per row: a power of two (others pack badly into the clusters' groups of SMs: 48 rows of
+    // 32000, 6 CTAs 43.2, 4 32.3), as many as leave every row's cluster resident at once, but no
+    // slices under 3 KB, where exchanges cost more than the slices save, and enough for slices of
+    // 64 KB, two of which fit an SM. What is resident at once was measured: 30 clusters of 8, 68 of 4,
+    // 148 of 2. Measured (us, sums over three kinds of filters, bf16 unless said): 32 rows of
+    // 1000: 1 CTA 23.2, 8 30.3; 8 of 8000: 4 20.8, 8 21.5, 1 23.5; 28 of 32000: 8 30.1, 4 31.3; 36 of
+    // 32000: 4 31.3, 2 33.7, 8 41.3; 74: 2 33.6, 4 44.8; 256 of 32000: 1 73.9, 2 76.6; 256 of 131072, top-k
+    // and top-p: 4 48.6, 2 54.7, 8 66.9. A few rows more than are resident at once cost less than twice
+    // as long slices where those are long (33 of 50257 f32, mixed filters and masks: 8 16.3, 4 18.2; of
+    // 131072 f32: 56.8 and 60.8; of 32000 f32: 35.9 and 31.4; 36 of 50257 f32: 47.6 and 41.2).
+    const int fit = a.rows <= (bytes > 160 * 1024 ? 33 : 30) ? 8 : a.rows <= 68 ? 4 : a.rows <= 148 ? 2 : 1;
+    int need = 1, most = 1;
+    while (need < kMostCtas && bytes > need * 65536) need *= 2;
+    while (most < kMostCtas && bytes >= 2 * most * 3072) most *= 2;
+    const int ctas = std::max(need, std::min(fit, most));
     const size_t smem = std::max<size_t>((size_t)(((a.vocab + kVec<T> - 1) / kVec<T> + ctas - 1) / ctas) * 16, 2 * kList * 8);
     static bool ready[64] = {};
     int device = 0;
