@@ -823,21 +823,23 @@ sample_cluster_kernel(SampleArgs a, int shift, int ctas) {
 template <typename T>
 bool launch_cluster(const SampleArgs& a, int shift, cudaStream_t s) {
     const int64_t bytes = a.vocab * (int64_t)sizeof(T);
-    constexpr int64_t kMost = 200 * 1024;      // of a slice
+    constexpr int64_t kMost = 200 * 1024, kTwoFit = 100 * 1024;     // of a slice, and where two CTAs fit an SM
     if (bytes / kMostCtas > kMost) return false;
     // CTAs per row: a power of two (others pack badly into the clusters' groups of SMs: 48 rows of
     // 32000, 6 CTAs 43.2, 4 32.3), as many as leave every row's cluster resident at once, but no
     // slices under 3 KB, where exchanges cost more than the slices save, and enough for slices of
-    // 64 KB, two of which fit an SM. What is resident at once was measured: 30 clusters of 8, 68 of 4,
+    // 100 KB, two of which fit an SM. What is resident at once was measured: 30 clusters of 8, 68 of 4,
     // 148 of 2. Measured (us, sums over three kinds of filters, bf16 unless said): 32 rows of
     // 1000: 1 CTA 23.2, 8 30.3; 8 of 8000: 4 20.8, 8 21.5, 1 23.5; 28 of 32000: 8 30.1, 4 31.3; 36 of
-    // 32000: 4 31.3, 2 33.7, 8 41.3; 74: 2 33.6, 4 44.8; 256 of 32000: 1 73.9, 2 76.6; 256 of 131072, top-k
+    // 32000: 4 31.3, 2 33.7, 8 41.3; 74: 2 33.6, 4 44.8; 256 of 32000: 1 73.9, 2 76.6; 148 of 36000 f32: 2 58.8,
+    // 4 81.7; 256 of 50257 f32: 2 128.9, 4 148.8; 256 of 100001 f32: 4 229.4, 8 284.5; 256 of 131072, top-k
     // and top-p: 4 48.6, 2 54.7, 8 66.9. A few rows more than are resident at once cost less than twice
     // as long slices where those are long (33 of 50257 f32, mixed filters and masks: 8 16.3, 4 18.2; of
-    // 131072 f32: 56.8 and 60.8; of 32000 f32: 35.9 and 31.4; 36 of 50257 f32: 47.6 and 41.2).
-    const int fit = a.rows <= (bytes > 160 * 1024 ? 33 : 30) ? 8 : a.rows <= 68 ? 4 : a.rows <= 148 ? 2 : 1;
+    // 131072 f32: 56.8 and 60.8; of 32000 f32: 35.9 and 31.4; 36 of 50257 f32: 47.6 and 41.2; 100 of 100001:
+    // 4 101.0, 2 107.6; 148 of 100001: 135.8 and 120.3; 100 of 50257: 68.9 and 66.8).
+    const int fit = a.rows <= (bytes > 160 * 1024 ? 33 : 30) ? 8 : a.rows <= (a.vocab > 60000 ? 110 : 68) ? 4 : a.rows <= 148 ? 2 : 1;
     int need = 1, most = 1;
-    while (need < kMostCtas && bytes > need * 65536) need *= 2;
+    while (need < kMostCtas && bytes > need * kTwoFit) need *= 2;
     while (most < kMostCtas && bytes >= 2 * most * 3072) most *= 2;
     const int ctas = std::max(need, std::min(fit, most));
     const size_t smem = std::max<size_t>((size_t)(((a.vocab + kVec<T> - 1) / kVec<T> + ctas - 1) / ctas) * 16, 2 * kList * 8);
