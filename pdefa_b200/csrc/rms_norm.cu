@@ -449,13 +449,13 @@ __device__ __forceinline__ void by_offset(int s, F f) {
 // memory's own grid, which begins s columns before the row, are read and written as they are
 // and only the weights are shifted. A piece at the row's ends is read whole where the array goes
 // on beyond the row, and written by halves. The order in which the squares are added depends on s.
-// Bound by its instructions and its barriers, so registers are limited to what keeps three CTAs
-// of 544 threads on an SM (4000 x 8191 bf16, residual, 8-bit output: 60 us, the general kernel 84,
-// with one CTA on an SM 96; 4000 x 8190, 16-bit output: 51, general 84; 16000 x 2049, 8-bit: 51
-// against 57; 509 x 2050 f16: 2.6 against 3.0). Weights read early pay with one piece a thread only
-// (2.6 against 2.75; 55 against 51 with two).
+// Bound by its instructions and its barriers, so registers are limited, to 40 with two or three pieces
+// a thread, for two CTAs of 544 threads on an SM or four of 352 (4000 x 8191 bf16, residual, 8-bit output:
+// 54 us, over two pieces 59, with one CTA on an SM 96, the general kernel 84; 4000 x 8190, 16-bit
+// output: 43, general 84; 16000 x 2049, 8-bit: 50 against 57; 509 x 2050 f16: 2.6 against 3.0). Weights read
+// early pay with one piece a thread only (2.6 against 2.75; 55 against 51 with two).
 template <typename T, typename W, int N, bool QUANT>
-__global__ void __launch_bounds__(N == 2 ? 768 : 1024, N == 4 ? 1 : 2)
+__global__ void __launch_bounds__(N == 2 ? 768 : N == 3 ? 448 : 1024, N == 4 ? 1 : N == 3 ? 3 : 2)
 rms_norm_alike_kernel(RmsNormArgs a) {
     constexpr int P = kPiece<T>, PW = kPiece<W>, H = kGroup / P;
     using Q = typename BytePiece<P>::type;
@@ -624,14 +624,20 @@ void launch_n(const RmsNormArgs& a, int64_t pieces, cudaStream_t s) {
 // Pieces per thread: one where all rows run at once (550 x 4096 bf16, residual, 8-bit: 3.5 us, with
 // two 4.5; 509 x 2050 f16: 2.6 and 4.1), two for more rows (16384 x 8192: 139 us, one 182, four 142;
 // 500 x 6001: 6.4, one 8.2), four for rows that two do not hold.
+// Contiguous odd rows that do not run at once take three where that leaves fewer of the threads'
+// slots empty than two (4000 x 8190 bf16: 43.0, two 51.3; 16000 x 2050: 32.5 and 38.3; where it
+// does not: 8000 x 4001, 8-bit, 56.2 and 47.5; at once: 200 x 8191 7.7 and 5.0).
 template <typename T, typename W, bool QUANT, Rows ROWS>
 bool launch_pieces(const RmsNormArgs& a, cudaStream_t s) {
     const int64_t ends = ROWS == Rows::kAlike ? kPiece<T> - 1 : 0;      // columns before the row in its first piece
     const int64_t pieces = (a.cols + ends + kPiece<T> - 1) / kPiece<T>;
     if (pieces > 4 * 1024) return false;
     const int64_t most = ROWS == Rows::kAlike ? 768 : 1024;     // threads, with two pieces each
+    auto slots = [&](int64_t n) { return ((pieces + n - 1) / n + 31) / 32 * 32 * n; };      // of a CTA's threads, n each
     const bool at_once = a.rows * ((pieces + 31) / 32 * 32) <= 148 * 2048;
+    const bool three = ROWS == Rows::kAlike && !at_once && pieces <= 3 * 448 && slots(3) < slots(2);
     if (pieces > 2 * most) launch_n<T, W, 4, QUANT, ROWS>(a, pieces, s);
+    else if (three) launch_n<T, W, ROWS == Rows::kAlike ? 3 : 2, QUANT, ROWS>(a, pieces, s);
     else if (pieces > 1024 || (!at_once && pieces > 32)) launch_n<T, W, 2, QUANT, ROWS>(a, pieces, s);
     else launch_n<T, W, 1, QUANT, ROWS>(a, pieces, s);
     return true;

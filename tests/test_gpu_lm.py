@@ -95,7 +95,7 @@ def test_norm(rows, cols, dtype, residual, gap):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids)
-@pytest.mark.parametrize("rows,cols", [(9, 17), (40, 131), (13, 1031), (1100, 1153), (700, 3001), (9, 8191), (11, 13001),
+@pytest.mark.parametrize("rows,cols", [(9, 17), (40, 131), (13, 1031), (1100, 1153), (700, 3001), (1100, 2051), (1300, 1537), (9, 8191), (11, 13001),
                                        (7, 16383), (3, 32761)])
 def test_norm_rows_of_every_offset(rows, cols, dtype):
     """Contiguous rows of odd lengths start at every offset within 16 bytes; what lies beside a row stays out of it."""
