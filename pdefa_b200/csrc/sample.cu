@@ -61,6 +61,10 @@ __device__ __forceinline__ float value_of(uint64_t at, int shift) {
     return v == v ? v : -INFINITY;
 }
 
+// log2(e) / T, within the numbers: neither 0 * inf from an infinite T nor inf * 0 from one below 2^-127
+// may meet a difference of logits.
+__device__ __forceinline__ float factor(float temp) { return fminf(fmaxf(kLog2e / temp, 1.17549435e-38f), 3.40282347e38f); }
+
 struct Race {
     float key = -1.0f;
     uint32_t idx = 0xFFFFFFFFu;
@@ -138,7 +142,7 @@ sample_rows_kernel(SampleArgs a, int shift) {
         }
         return;
     }
-    const float c = kLog2e / temp;
+    const float c = factor(temp);
     auto weight = [&](float x) {
         if (x == mx) return 1.0f;              // also inf - inf
         if (x == -INFINITY) return 0.0f;
@@ -545,9 +549,7 @@ sample_cluster_kernel(SampleArgs a, int shift, int ctas) {
         top = 0.0f;
     }
 
-    // w = 2^y with y = (x - top) * log2(e) / T; the bound on the factor keeps -inf * 0 out
-    // (an infinite temperature).
-    const float c = fmaxf(kLog2e / temp, 1.17549435e-38f);
+    const float c = factor(temp);       // w = 2^y with y = (x - top) * log2(e) / T
     auto weight = [&](float x) { return ex2((x - top) * c); };
     auto finish = [&](uint32_t token, float x, float z) {
         a.tokens[row] = (int32_t)token;

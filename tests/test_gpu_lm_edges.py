@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 
 import pdefa_b200 as pb
+from test_gpu_lm import SETTINGS, check_sample, logits_of, noise_of
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -95,3 +96,32 @@ def test_norm_8bit_of_infinite_products(rows, cols):
     got, want = q.cpu().float(), want_q.float()
     assert torch.equal(got.isnan(), want.isnan()) and got[:, 130].isnan().all()
     assert torch.equal(got.nan_to_num(), want.nan_to_num())
+
+
+# rows that a cluster holds, and longer ones
+@pytest.mark.parametrize("vocab", [3001, 409701])
+@pytest.mark.parametrize("t", [1.5e-45, 1e-39, 4.2e-39, 1.1e-38, 1.2e-38, 3e38])
+def test_sample_extreme_temperatures(vocab, t):
+    """Temperatures whose inverse no 32-bit number holds: the largest logits share the mass, or all do."""
+    g = gen(vocab)
+    rows = len(SETTINGS)
+    x, e = logits_of(g, rows, vocab, torch.float32), noise_of(g, rows, vocab)
+    x[1::2] = torch.round(x[1::2])                # several largest
+    x[2::4, ::2] = -float("inf")
+    tok, prob = check_sample(x, e, t=[t] * rows, k=[s.get("k", 0) for s in SETTINGS], p=[s.get("p", 1.0) for s in SETTINGS],
+                             m=[s.get("m", 0.0) for s in SETTINGS])
+    assert prob.isfinite().all() and (prob > 0).all()
+    if t < 1:
+        assert torch.equal(x.gather(1, tok[:, None].long())[:, 0], x.amax(1))
+
+
+@pytest.mark.parametrize("vocab", [3001, 409701])
+def test_sample_infinite_temperature(vocab):
+    g = gen(vocab)
+    x, e = logits_of(g, 3, vocab, torch.float32), noise_of(g, 3, vocab)
+    x[1, ::3] = -float("inf")                     # ruled out at any temperature
+    x[2, [70, 1000, 2900]] = float("inf")         # these alone share the mass
+    tok, prob = pb.ops_sample(x, e, temperature=torch.full((3,), float("inf"), device="cuda"))
+    left = torch.stack([torch.ones(vocab, dtype=torch.bool, device="cuda"), x[1] > -float("inf"), x[2] == float("inf")])
+    assert torch.equal(tok.long(), torch.where(left, e, torch.inf).argmin(1))
+    assert torch.allclose(prob, 1 / left.sum(1).float(), rtol=1e-5)
