@@ -265,8 +265,8 @@ ENGINE_API EngineStatus engine_matmul_grouped_fp8_device(const void* d_a, int64_
  * before it, the mass before it is below top_p * Z, w >= min_p and w > 0; the first
  * token is always kept. Of the kept tokens the one with the largest w / noise wins
  * (lowest index among equals): with noise [rows, vocab] of independent exponential
- * variates, token i is drawn with probability w_i / (sum of kept w). Negative or NaN
- * noise takes its token out of the race.
+ * variates, token i is drawn with probability w_i / (sum of kept w). Negative (-0
+ * too) or NaN noise takes its token out of the race.
  * d_temperature, d_top_k, d_top_p, d_min_p: one value per row, or NULL (1, off, off,
  * off). A temperature that is not above 0 picks the first token; top_k <= 0, top_p >= 1
  * and min_p <= 0 are off. d_tokens[row]: the token, -1 where every logit is -inf;

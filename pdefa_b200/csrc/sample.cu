@@ -65,6 +65,10 @@ __device__ __forceinline__ float value_of(uint64_t at, int shift) {
 // may meet a difference of logits.
 __device__ __forceinline__ float factor(float temp) { return fminf(fmaxf(kLog2e / temp, 1.17549435e-38f), 3.40282347e38f); }
 
+// A variate that races: not NaN and without a sign. -0, which -log(1 - u) gives for u = 0, would make
+// w / e negative.
+__device__ __forceinline__ bool races(float e) { return __float_as_uint(e) <= 0x7F800000u; }
+
 struct Race {
     float key = -1.0f;
     uint32_t idx = 0xFFFFFFFFu;
@@ -178,7 +182,7 @@ sample_rows_kernel(SampleArgs a, int shift) {
             const float w = weight(x);
             if (!(w >= floor_w && w > 0.0f) && i != first) continue;
             const float e = noise[i];
-            if (e >= 0.0f) r.take(w / e, i, x);
+            if (races(e)) r.take(w / e, i, x);
         }
         r = warp_race(r);
         __syncthreads();
@@ -440,7 +444,7 @@ __device__ __forceinline__ uint4 choose(Shared& sh, uint64_t* at_of, int n, int 
     if (i < n && tid % g == 0) {
         if (before == 0) sh.first = own.y;
         const bool kept = before == 0 || ((int)before < k && (!by_mass || (double)mass < (double)limit * 1099511627776.0));
-        if (kept && e >= 0.0f)
+        if (kept && races(e))
             race = make_uint4(__float_as_uint(__fdividef(ex2((__uint_as_float(own.x) - top) * c), e)) + 1, own.y, own.x, 0);
     }
     race = JoinRace::warp(race);
@@ -587,7 +591,7 @@ sample_cluster_kernel(SampleArgs a, int shift, int ctas) {
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    if (!(e[u][j] >= 0.0f)) continue;
+                    if (!races(e[u][j])) continue;
                     const uint32_t key = __float_as_uint(__fdividef(wx[u][j], e[u][j])) + 1;
                     const uint32_t i = (v0 + v + u * kSlice) * VEC + j;
                     if (key > race.x || (key == race.x && i < race.y)) {

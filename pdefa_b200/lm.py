@@ -82,7 +82,8 @@ def ops_sample(logits, noise, temperature=None, top_k=None, top_p=None, min_p=No
     """One token per row of logits -> (tokens int32 [rows], probs float32 [rows]).
 
     logits [rows, vocab] float32, float16 or bfloat16 (-inf: ruled out); noise [rows,
-    vocab] float32 of independent exponential variates (Tensor.exponential_()).
+    vocab] float32 of independent exponential variates (Tensor.exponential_()); a token whose
+    variate is negative, -0 or NaN is out of the race.
     temperature, top_p, min_p float32 [rows] and top_k int32 [rows], each optional:
     temperature 0 takes the largest logit, top_k <= 0, top_p >= 1 and min_p <= 0 are off.
     With w = exp((logit - largest) / temperature) a token is kept if fewer than top_k

@@ -125,3 +125,23 @@ def test_sample_infinite_temperature(vocab):
     left = torch.stack([torch.ones(vocab, dtype=torch.bool, device="cuda"), x[1] > -float("inf"), x[2] == float("inf")])
     assert torch.equal(tok.long(), torch.where(left, e, torch.inf).argmin(1))
     assert torch.allclose(prob, 1 / left.sum(1).float(), rtol=1e-5)
+
+
+@pytest.mark.parametrize("vocab", [3001, 409701])
+def test_sample_negative_zero_noise(vocab):
+    """w / -0 is -inf: the token loses, in every kind of row; against +0 too."""
+    g = gen(vocab)
+    n = len(SETTINGS)
+    x, e = logits_of(g, 4 * n, vocab, torch.float32), noise_of(g, 4 * n, vocab)
+    at = torch.arange(n, device="cuda")
+    e[at, x[:n].argmax(1)] = -0.0
+    e[n:2 * n, 100::2] = -0.0
+    e[2 * n:3 * n] = -0.0                         # no usable variate: the first token
+    top = x[3 * n:].topk(2, dim=1).indices
+    e[3 * n + at, top[:, 0]] = -0.0
+    e[3 * n + at, top[:, 1]] = 0.0
+    every = 4 * SETTINGS
+    tok, _ = check_sample(x, e, t=[s.get("t", 1.0) for s in every], k=[s.get("k", 0) for s in every],
+                          p=[s.get("p", 1.0) for s in every], m=[s.get("m", 0.0) for s in every])
+    assert torch.equal(tok[2 * n:3 * n].long(), x[2 * n:3 * n].argmax(1))
+    assert tok[3 * n] == top[0, 1]                # no filter: the one with +0
