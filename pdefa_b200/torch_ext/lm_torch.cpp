@@ -111,11 +111,13 @@ PyObject* guarded(F&& f) {
     END_HANDLE_TH_ERRORS
 }
 
-template <class F>
-int unlocked(F&& f) {
+// Calls a C entry point without the interpreter's lock. The arguments are made before: pointers
+// of tensors without storage (fake ones, under tracing) and streams throw, which needs the lock.
+template <class F, class... A>
+int unlocked(F f, A... a) {
     int rc;
     Py_BEGIN_ALLOW_THREADS
-    rc = (int)f();
+    rc = (int)f(a...);
     Py_END_ALLOW_THREADS
     return rc;
 }
@@ -172,12 +174,10 @@ PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
             y = at::empty(x.sizes(), x.options().requires_grad(false));
         }
         if (rx.rows > 0 && rx.cols > 0) {
-            const int rc = unlocked([&] {
-                return g_rms_norm(x.const_data_ptr(), rx.stride, res ? res->const_data_ptr() : nullptr, rr.stride, w.const_data_ptr(),
-                                  res ? h.mutable_data_ptr() : nullptr, rx.cols, y.mutable_data_ptr(), rx.cols,
-                                  fp8 ? scales.mutable_data_ptr<float>() : nullptr, nb, rx.rows, rx.cols, code,
-                                  float_code(w.scalar_type()), (float)eps, device, stream_of(device));
-            });
+            const int rc = unlocked(g_rms_norm, x.const_data_ptr(), rx.stride, res ? res->const_data_ptr() : nullptr, rr.stride,
+                                    w.const_data_ptr(), res ? h.mutable_data_ptr() : nullptr, rx.cols, y.mutable_data_ptr(), rx.cols,
+                                    fp8 ? scales.mutable_data_ptr<float>() : nullptr, nb, rx.rows, rx.cols, code,
+                                    float_code(w.scalar_type()), (float)eps, device, stream_of(device));
             if (rc) return status(rc, op);
         } else if (!(eps >= 0.0 && eps <= 3.4e38)) {
             refuse(op, "eps must be finite and >= 0");
@@ -229,15 +229,15 @@ PyObject* matmul(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const at::ScalarType type = out_type(args[GROUPED ? 5 : 4], op, &code);
         if (GROUPED && experts == 0) return THPVariable_Wrap(at::zeros({m, nn}, a.options().dtype(type)));
         at::Tensor out = at::empty({m, nn}, a.options().dtype(type).requires_grad(false));
-        const int rc = unlocked([&]() -> int {
-            if (GROUPED)
-                return g_grouped(a.const_data_ptr(), a.stride(0), sa.const_data_ptr<float>(), sa.stride(0), b.const_data_ptr(), b.stride(1),
-                                 b.stride(0), sb.const_data_ptr<float>(), sb.stride(1), sb.stride(0), off->const_data_ptr<int32_t>(),
-                                 experts, out.mutable_data_ptr(), nn, code, m, nn, k, device, stream_of(device));
-            return g_matmul(a.const_data_ptr(), a.stride(0), sa.const_data_ptr<float>(), sa.stride(0), b.const_data_ptr(), b.stride(0),
-                            sb.const_data_ptr<float>(), sb.stride(0), out.mutable_data_ptr(), nn, code, m, nn, k, device,
-                            stream_of(device));
-        });
+        int rc;
+        if constexpr (GROUPED)
+            rc = unlocked(g_grouped, a.const_data_ptr(), a.stride(0), sa.const_data_ptr<float>(), sa.stride(0), b.const_data_ptr(),
+                          b.stride(1), b.stride(0), sb.const_data_ptr<float>(), sb.stride(1), sb.stride(0),
+                          off->const_data_ptr<int32_t>(), experts, out.mutable_data_ptr(), nn, code, m, nn, k, device, stream_of(device));
+        else
+            rc = unlocked(g_matmul, a.const_data_ptr(), a.stride(0), sa.const_data_ptr<float>(), sa.stride(0), b.const_data_ptr(),
+                          b.stride(0), sb.const_data_ptr<float>(), sb.stride(0), out.mutable_data_ptr(), nn, code, m, nn, k, device,
+                          stream_of(device));
         if (rc) return status(rc, op);
         return THPVariable_Wrap(std::move(out));
     });
@@ -267,12 +267,10 @@ PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t n) {
         }
         at::Tensor tokens = at::empty({rows}, x.options().dtype(at::kInt).requires_grad(false));
         at::Tensor probs = at::empty({rows}, x.options().dtype(at::kFloat).requires_grad(false));
-        const int rc = unlocked([&] {
-            return g_sample(x.const_data_ptr(), x.stride(0), code, e.const_data_ptr<float>(), e.stride(0),
-                            static_cast<const float*>(per_row[0]), static_cast<const int32_t*>(per_row[1]),
-                            static_cast<const float*>(per_row[2]), static_cast<const float*>(per_row[3]), rows, vocab,
-                            tokens.mutable_data_ptr<int32_t>(), probs.mutable_data_ptr<float>(), device, stream_of(device));
-        });
+        const int rc = unlocked(g_sample, x.const_data_ptr(), x.stride(0), code, e.const_data_ptr<float>(), e.stride(0),
+                                static_cast<const float*>(per_row[0]), static_cast<const int32_t*>(per_row[1]),
+                                static_cast<const float*>(per_row[2]), static_cast<const float*>(per_row[3]), rows, vocab,
+                                tokens.mutable_data_ptr<int32_t>(), probs.mutable_data_ptr<float>(), device, stream_of(device));
         if (rc) return status(rc, op);
         return Py_BuildValue("NN", THPVariable_Wrap(std::move(tokens)), THPVariable_Wrap(std::move(probs)));
     });
