@@ -4,8 +4,9 @@ The library is built in-tree (objects under pdefa_b200/_build, the shared object
 under pdefa_b200/lib) for sm_100a only. Only the C-ABI entry points are exported
 (-fvisibility=hidden + explicit default visibility on the API declarations).
 
-Where torch is installed, lib/lm_torch.so (pdefa_b200/torch_ext) is built too: the
-binding of the language-model operators for torch tensors.
+Where a torch with CUDA is installed, lib/lm_torch.so (pdefa_b200/torch_ext) is built too:
+the binding of the language-model operators for torch tensors. The engine does without it:
+if it cannot be built, build() warns, and the first call of such an operator says why.
 
 Usage: python -m pdefa_b200.build [--force] [--jobs N]
 """
@@ -19,6 +20,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 SRC = os.path.join(HERE, "csrc")
@@ -63,8 +65,10 @@ def compile_one(src: str, force: bool) -> str:
 
 
 def build_torch_binding(force: bool) -> None:
+    """Builds TORCH_LIB unless it is up to date or there is no torch with CUDA to bind. Raises
+    RuntimeError with the compiler's output."""
     spec = importlib.util.find_spec("torch")
-    if spec is None or not spec.origin:
+    if spec is None or not spec.origin or not os.path.exists(os.path.join(os.path.dirname(spec.origin), "lib", "libc10_cuda.so")):
         return
     if (not force and os.path.exists(TORCH_LIB)
             and os.path.getmtime(TORCH_LIB) >= max(os.path.getmtime(TORCH_SRC), _newest_header())):
@@ -76,7 +80,10 @@ def build_torch_binding(force: bool) -> None:
     cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", *("-I" + i for i in inc), TORCH_SRC,
            "-o", TORCH_LIB + ".tmp", "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
            "-ltorch_python"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
+    try:
+        r = subprocess.run(cmd, capture_output=True, text=True)
+    except OSError as e:
+        raise RuntimeError(f"torch binding: {e}") from e
     if r.returncode != 0:
         raise RuntimeError(f"torch binding failed:\n{r.stdout}\n{r.stderr}")
     os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
@@ -90,7 +97,6 @@ def build(force: bool = False, jobs: int = 0) -> str:
     with cf.ThreadPoolExecutor(jobs) as ex:
         binding = ex.submit(build_torch_binding, force)
         objs = list(ex.map(lambda s: compile_one(s, force), srcs))
-        binding.result()
     if (force or not os.path.exists(LIB)
             or max(os.path.getmtime(o) for o in objs) > os.path.getmtime(LIB)):
         cmd = [nvcc(), "-shared", *ARCH, "-cudart", "static", "-o", LIB + ".tmp", *objs, "-lpthread", "-ldl", "-lrt", "-lz"]
@@ -98,6 +104,10 @@ def build(force: bool = False, jobs: int = 0) -> str:
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         os.replace(LIB + ".tmp", LIB)
+    try:
+        binding.result()
+    except RuntimeError as e:
+        warnings.warn(f"the language-model operators have no binding for torch tensors: {e}", RuntimeWarning, stacklevel=2)
     return LIB
 
 

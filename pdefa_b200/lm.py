@@ -37,7 +37,9 @@ def _binding():
         from . import build
         lib = N.lib()
         if not os.path.isfile(build.TORCH_LIB):
-            build.build_torch_binding(False)
+            build.build_torch_binding(False)        # raises RuntimeError with the compiler's output
+            if not os.path.isfile(build.TORCH_LIB):
+                raise TypeError("the language-model operators take CUDA torch tensors: this torch has no CUDA")
         loader = importlib.machinery.ExtensionFileLoader("lm_torch", build.TORCH_LIB)
         b = importlib.util.module_from_spec(importlib.util.spec_from_loader("lm_torch", loader))
         loader.exec_module(b)

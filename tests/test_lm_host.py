@@ -1,9 +1,13 @@
 """The host side of the language-model operators, without a GPU."""
+import importlib.machinery
+import importlib.util
 import os
 import subprocess
 import sys
 
 import pytest
+
+from pdefa_b200 import build, lm
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -34,3 +38,55 @@ def test_tensors_without_storage_are_refused():
                        env={**os.environ, "PYTHONPATH": ROOT})
     assert r.returncode == 0, r.stderr[-2000:]
     assert r.stdout.split() == ["refused"] * 7
+
+
+@pytest.fixture
+def odd_torch(tmp_path, monkeypatch):
+    """What build() sees as the installed torch: a package with CUDA but without headers; outputs go to tmp_path."""
+    (tmp_path / "torch" / "lib").mkdir(parents=True)
+    (tmp_path / "torch" / "__init__.py").write_text("")
+    (tmp_path / "torch" / "version.py").write_text("__version__ = '0.0.1+none'\n")
+    (tmp_path / "torch" / "lib" / "libc10_cuda.so").write_text("")
+    find = importlib.util.find_spec
+    spec = importlib.machinery.ModuleSpec("torch", None, origin=str(tmp_path / "torch" / "__init__.py"))
+    monkeypatch.setattr(importlib.util, "find_spec", lambda name, *a: spec if name == "torch" else find(name, *a))
+    monkeypatch.setattr(build, "TORCH_LIB", str(tmp_path / "lm_torch.so"))
+    monkeypatch.setattr(build, "LIB", str(tmp_path / "libpdefa_native.so"))
+    monkeypatch.setattr(build, "LIB_DIR", str(tmp_path))
+    return tmp_path
+
+
+def test_engine_builds_without_the_binding(odd_torch):
+    with pytest.warns(RuntimeWarning, match="no binding for torch"):
+        assert build.build() == str(odd_torch / "libpdefa_native.so")
+    assert (odd_torch / "libpdefa_native.so").stat().st_size > 1000000
+    assert not (odd_torch / "lm_torch.so").exists()
+
+
+def test_engine_builds_without_a_compiler_for_the_binding(odd_torch, monkeypatch):
+    run = subprocess.run
+
+    def no_gxx(cmd, **kw):
+        if cmd[0] == "g++":
+            raise FileNotFoundError("g++")
+        return run(cmd, **kw)
+
+    monkeypatch.setattr(subprocess, "run", no_gxx)
+    with pytest.warns(RuntimeWarning, match="g\\+\\+"):
+        assert os.path.exists(build.build())
+
+
+def test_torch_without_cuda_has_no_binding(odd_torch, monkeypatch, recwarn):
+    pytest.importorskip("torch")
+    (odd_torch / "torch" / "lib" / "libc10_cuda.so").unlink()
+    assert os.path.exists(build.build()) and not recwarn.list
+    monkeypatch.setattr(lm, "_B", None)
+    with pytest.raises(TypeError, match="no CUDA"):
+        lm.ops_sample(None, None)
+
+
+def test_first_call_says_why_there_is_no_binding(odd_torch, monkeypatch):
+    pytest.importorskip("torch")
+    monkeypatch.setattr(lm, "_B", None)
+    with pytest.raises(RuntimeError, match="torch binding failed"):
+        lm.ops_sample(None, None)
