@@ -4,8 +4,9 @@ The library is built in-tree (objects under pdefa_b200/_build, the shared object
 under pdefa_b200/lib) for sm_100a only. Only the C-ABI entry points are exported
 (-fvisibility=hidden + explicit default visibility on the API declarations).
 
-Where a torch with CUDA is installed, lib/lm_torch.so (pdefa_b200/torch_ext) is built too:
-the binding of the language-model operators for torch tensors. The engine does without it:
+Where a torch with CUDA is installed, lib/lm_torch-<python>-<torch>.so (pdefa_b200/torch_ext)
+is built too: the binding of the language-model operators for torch tensors. It fits these
+versions only, so they are part of its name. The engine does without it:
 if it cannot be built, build() warns, and the first call of such an operator says why.
 
 Usage: python -m pdefa_b200.build [--force] [--jobs N]
@@ -16,6 +17,7 @@ import argparse
 import concurrent.futures as cf
 import importlib.util
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -28,7 +30,6 @@ BUILD = os.path.join(HERE, "_build")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIB_DIR, "libpdefa_native.so")
 TORCH_SRC = os.path.join(HERE, "torch_ext", "lm_torch.cpp")
-TORCH_LIB = os.path.join(LIB_DIR, "lm_torch.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -64,21 +65,39 @@ def compile_one(src: str, force: bool) -> str:
     return obj
 
 
-def build_torch_binding(force: bool) -> None:
-    """Builds TORCH_LIB unless it is up to date or there is no torch with CUDA to bind. Raises
-    RuntimeError with the compiler's output."""
+def torch_root():
+    """The installed torch's folder; None without torch or where it has no CUDA."""
     spec = importlib.util.find_spec("torch")
-    if spec is None or not spec.origin or not os.path.exists(os.path.join(os.path.dirname(spec.origin), "lib", "libc10_cuda.so")):
-        return
-    if (not force and os.path.exists(TORCH_LIB)
-            and os.path.getmtime(TORCH_LIB) >= max(os.path.getmtime(TORCH_SRC), _newest_header())):
-        return
+    if spec is None or not spec.origin:
+        return None
     root = os.path.dirname(spec.origin)
+    return root if os.path.exists(os.path.join(root, "lib", "libc10_cuda.so")) else None
+
+
+def torch_lib(root: str) -> str:
+    """The binding for this Python and the torch at `root`, whose version is read without importing it."""
+    with open(os.path.join(root, "version.py")) as f:
+        found = re.search(r"^__version__\s*=\s*['\"]([\w.+-]+)['\"]", f.read(), re.M)
+    if not found:
+        raise RuntimeError(f"torch binding: no version in {f.name}")
+    return os.path.join(LIB_DIR, f"lm_torch-{sys.implementation.cache_tag}-{found.group(1)}.so")
+
+
+def build_torch_binding(force: bool) -> None:
+    """Builds torch_lib() unless it is up to date or there is no torch with CUDA to bind. Raises
+    RuntimeError with the compiler's output."""
+    root = torch_root()
+    if root is None:
+        return
+    lib = torch_lib(root)
+    if (not force and os.path.exists(lib)
+            and os.path.getmtime(lib) >= max(os.path.getmtime(TORCH_SRC), _newest_header())):
+        return
     cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")
     inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
            sysconfig.get_paths()["include"], cuda]
     cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", *("-I" + i for i in inc), TORCH_SRC,
-           "-o", TORCH_LIB + ".tmp", "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
+           "-o", lib + ".tmp", "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
            "-ltorch_python"]
     try:
         r = subprocess.run(cmd, capture_output=True, text=True)
@@ -86,7 +105,7 @@ def build_torch_binding(force: bool) -> None:
         raise RuntimeError(f"torch binding: {e}") from e
     if r.returncode != 0:
         raise RuntimeError(f"torch binding failed:\n{r.stdout}\n{r.stderr}")
-    os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
+    os.replace(lib + ".tmp", lib)
 
 
 def build(force: bool = False, jobs: int = 0) -> str:

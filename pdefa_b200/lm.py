@@ -10,7 +10,7 @@ tensor, a wrong dtype) or PdefaError (shapes, strides). There are no gradients: 
 only infers. The kernels' device-side waits are bounded; one that runs out is recorded in
 the device's error word (engine_device_error).
 
-The argument checks and the calls are in lib/lm_torch.so (torch_ext/lm_torch.cpp).
+The argument checks and the calls are in lib/lm_torch-*.so (torch_ext/lm_torch.cpp).
 """
 from __future__ import annotations
 
@@ -29,18 +29,20 @@ _B = None
 
 
 def _binding():
-    """lm_torch.so, bound to the engine's entry points."""
+    """The binding of the installed torch, bound to the engine's entry points."""
     global _B
     if _B is None:
         if "torch" not in sys.modules:
             raise TypeError("the language-model operators take CUDA torch tensors")
         from . import build
         lib = N.lib()
-        if not os.path.isfile(build.TORCH_LIB):
+        root = build.torch_root()
+        if root is None:
+            raise TypeError("the language-model operators take CUDA torch tensors: this torch has no CUDA")
+        path = build.torch_lib(root)
+        if not os.path.isfile(path):
             build.build_torch_binding(False)        # raises RuntimeError with the compiler's output
-            if not os.path.isfile(build.TORCH_LIB):
-                raise TypeError("the language-model operators take CUDA torch tensors: this torch has no CUDA")
-        loader = importlib.machinery.ExtensionFileLoader("lm_torch", build.TORCH_LIB)
+        loader = importlib.machinery.ExtensionFileLoader("lm_torch", path)
         b = importlib.util.module_from_spec(importlib.util.spec_from_loader("lm_torch", loader))
         loader.exec_module(b)
         address = lambda f: C.cast(f, C.c_void_p).value   # noqa: E731

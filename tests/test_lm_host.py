@@ -50,7 +50,6 @@ def odd_torch(tmp_path, monkeypatch):
     find = importlib.util.find_spec
     spec = importlib.machinery.ModuleSpec("torch", None, origin=str(tmp_path / "torch" / "__init__.py"))
     monkeypatch.setattr(importlib.util, "find_spec", lambda name, *a: spec if name == "torch" else find(name, *a))
-    monkeypatch.setattr(build, "TORCH_LIB", str(tmp_path / "lm_torch.so"))
     monkeypatch.setattr(build, "LIB", str(tmp_path / "libpdefa_native.so"))
     monkeypatch.setattr(build, "LIB_DIR", str(tmp_path))
     return tmp_path
@@ -60,7 +59,7 @@ def test_engine_builds_without_the_binding(odd_torch):
     with pytest.warns(RuntimeWarning, match="no binding for torch"):
         assert build.build() == str(odd_torch / "libpdefa_native.so")
     assert (odd_torch / "libpdefa_native.so").stat().st_size > 1000000
-    assert not (odd_torch / "lm_torch.so").exists()
+    assert not list(odd_torch.glob("lm_torch*.so"))
 
 
 def test_engine_builds_without_a_compiler_for_the_binding(odd_torch, monkeypatch):
@@ -90,3 +89,25 @@ def test_first_call_says_why_there_is_no_binding(odd_torch, monkeypatch):
     monkeypatch.setattr(lm, "_B", None)
     with pytest.raises(RuntimeError, match="torch binding failed"):
         lm.ops_sample(None, None)
+
+
+def test_binding_is_of_the_installed_versions(odd_torch, monkeypatch):
+    """One that was built for another torch or Python is not taken, however new it is."""
+    pytest.importorskip("torch")
+    root = str(odd_torch / "torch")
+    first = build.torch_lib(root)
+    open(first, "w").close()
+    (odd_torch / "torch" / "version.py").write_text("__version__ = '0.0.2'\ndebug = False\n")
+    second = build.torch_lib(root)
+    monkeypatch.setattr(sys.implementation, "cache_tag", "cpython-399")
+    assert len({first, second, build.torch_lib(root)}) == 3
+    monkeypatch.setattr(lm, "_B", None)
+    with pytest.raises(RuntimeError, match="torch binding failed"):      # it is built, not loaded
+        lm.ops_sample(None, None)
+
+
+def test_loaded_binding_is_the_installed_versions_own():
+    torch = pytest.importorskip("torch")
+    with pytest.raises(TypeError):
+        lm.ops_sample(None, None)
+    assert torch.__version__ in lm._B.__spec__.loader.path and sys.implementation.cache_tag in lm._B.__spec__.loader.path
