@@ -276,6 +276,9 @@ ENGINE_API EngineStatus engine_sample_device(const void* d_logits, int64_t logit
                                              const int32_t* d_top_k, const float* d_top_p, const float* d_min_p,
                                              int64_t rows, int64_t vocab, int32_t* d_tokens, float* d_probs,
                                              int32_t device, void* stream);
+/* For tests and measurements, without a GPU: the CTAs that engine_sample_device takes per
+ * row, 1 to 8 that keep it in their shared memory, or 0 for one that reads it in every pass. */
+ENGINE_API EngineStatus engine_sample_plan(int64_t rows, int64_t vocab, int32_t dtype, int32_t* ctas);
 
 #ifdef __cplusplus
 }

@@ -195,4 +195,16 @@ ENGINE_API EngineStatus engine_sample_device(const void* d_logits, int64_t logit
     });
 }
 
+ENGINE_API EngineStatus engine_sample_plan(int64_t rows, int64_t vocab, int32_t dtype, int32_t* ctas) {
+    return guarded([&]() -> EngineStatus {
+        clear_error();
+        need_extent(rows, "sample: bad number of rows");
+        need(vocab >= 1 && vocab <= kMaxExtent, ENGINE_ERR_INVALID_SHAPE, "sample: a row needs 1 to 2^31 - 1 logits");
+        need(float_type(dtype), ENGINE_ERR_INVALID_ARG, "sample: dtype must be F32, F16 or BF16");
+        need(ctas != nullptr, ENGINE_ERR_NULL_PTR, "sample: nowhere to put the plan");
+        *ctas = sample_plan(rows, vocab, dtype);
+        return ENGINE_OK;
+    });
+}
+
 }  // extern "C"

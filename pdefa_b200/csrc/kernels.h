@@ -252,5 +252,7 @@ struct SampleArgs {
     int dtype = 0;
 };
 void launch_sample(const SampleArgs& a, cudaStream_t s);
+// CTAs that launch_sample takes per row: 1 to 8 in a cluster, 0: one that reads the row in every pass.
+int sample_plan(int64_t rows, int64_t vocab, int dtype);
 
 }  // namespace pb

@@ -826,28 +826,35 @@ sample_cluster_kernel(SampleArgs a, int shift, int ctas) {
     if (rank == 0 && tid == 0) finish(won.y, __uint_as_float(won.z), z);
 }
 
-template <typename T>
-bool launch_cluster(const SampleArgs& a, int shift, cudaStream_t s) {
-    const int64_t bytes = a.vocab * (int64_t)sizeof(T);
-    constexpr int64_t kMost = 200 * 1024, kTwoFit = 100 * 1024;     // of a slice, and where two CTAs fit an SM
-    if (bytes / kMostCtas > kMost) return false;
-    // CTAs per row: a power of two (others pack badly into the clusters' groups of SMs: 48 rows of
-    // 32000, 6 CTAs 43.2, 4 32.3), as many as leave every row's cluster resident at once, but no
-    // slices under 3 KB, where exchanges cost more than the slices save, and enough for slices of
-    // 100 KB, two of which fit an SM. What is resident at once was measured: 30 clusters of 8, 68 of 4,
-    // 148 of 2. Measured (us, sums over three kinds of filters, bf16 unless said): 32 rows of
-    // 1000: 1 CTA 23.2, 8 30.3; 8 of 8000: 4 20.8, 8 21.5, 1 23.5; 28 of 32000: 8 30.1, 4 31.3; 36 of
-    // 32000: 4 31.3, 2 33.7, 8 41.3; 74: 2 33.6, 4 44.8; 256 of 32000: 1 73.9, 2 76.6; 148 of 36000 f32: 2 58.8,
-    // 4 81.7; 256 of 50257 f32: 2 128.9, 4 148.8; 256 of 100001 f32: 4 229.4, 8 284.5; 256 of 131072, top-k
-    // and top-p: 4 48.6, 2 54.7, 8 66.9. A few rows more than are resident at once cost less than twice
-    // as long slices where those are long (33 of 50257 f32, mixed filters and masks: 8 16.3, 4 18.2; of
-    // 131072 f32: 56.8 and 60.8; of 32000 f32: 35.9 and 31.4; 36 of 50257 f32: 47.6 and 41.2; 100 of 100001:
-    // 4 101.0, 2 107.6; 148 of 100001: 135.8 and 120.3; 100 of 50257: 68.9 and 66.8).
-    const int fit = a.rows <= (bytes > 160 * 1024 ? 33 : 30) ? 8 : a.rows <= (a.vocab > 60000 ? 110 : 68) ? 4 : a.rows <= 148 ? 2 : 1;
+constexpr int64_t kMost = 200 * 1024, kTwoFit = 100 * 1024;     // bytes of a slice, and where two CTAs fit an SM
+
+// CTAs per row, 0 where no cluster holds it: a power of two (others pack badly into the clusters'
+// groups of SMs: 48 rows of 32000, 6 CTAs 43.2, 4 32.3), as many as leave every row's cluster resident
+// at once, but no slices under 3 KB, where exchanges cost more than the slices save, and enough for
+// slices of 100 KB, two of which fit an SM. A B200 holds 33 clusters of 8, 71 of 4 and 148 of 2; the last
+// few share SMs with all others, so the limits are 30 and 68. Measured (us, sums over three kinds of filters,
+// bf16 unless said), 8 CTAs against 4: 30 rows of 16000 26.2, 26.0; of 32000 28.9, 30.2; of 50257 36.2, 42.4;
+// 33 rows of 16000 32.3, 26.1; of 32000 34.2, 30.2; of 40000 f32 37.5, 33.6; of 50257 40.8, 42.2; of 80000 45.9,
+// 44.0; of 100001 50.6, 54.9; 34 of 50257 45.6, 42.1; 36 of 100001 57.3, 54.1. 4 against 2: 68 rows of 8000 28.7, 30.2;
+// of 32000 33.8, 38.6; 71 of 8000 32.1, 30.0; of 32000 35.7, 38.1; 72 of 32000 43.8, 38.0; 148 of 36000 f32 81.7,
+// 58.8. From 80000 tokens on half the rows may wait instead: 72 of 80000 68.8, 76.2; 110 of 80000 86.4, 94.9; 100
+// of 100001 100.0, 111.9; 148 of 100001 134.1, 128.2; but 72 of 64000 53.0, 51.6; 110 of 64000 74.1, 63.9. 2 against 1:
+// 256 of 32000 76.6, 73.9. Longer slices than need be: 256 of 50257 f32: 2 128.9, 4 148.8; 256 of 100001 f32:
+// 4 229.4, 8 284.5; 256 of 131072, top-k and top-p: 4 48.6, 2 54.7, 8 66.9; 32 of 1000: 1 23.2, 8 30.3; 8 of 8000: 4 20.8, 8 21.5.
+int ctas_per_row(int64_t rows, int64_t vocab, int64_t size) {
+    const int64_t bytes = vocab * size;
+    if (bytes / kMostCtas > kMost) return 0;
+    const int fit = rows <= 30 ? 8 : rows <= (vocab >= 80000 ? 110 : 68) ? 4 : rows <= 148 ? 2 : 1;
     int need = 1, most = 1;
     while (need < kMostCtas && bytes > need * kTwoFit) need *= 2;
     while (most < kMostCtas && bytes >= 2 * most * 3072) most *= 2;
-    const int ctas = std::max(need, std::min(fit, most));
+    return std::max(need, std::min(fit, most));
+}
+
+template <typename T>
+bool launch_cluster(const SampleArgs& a, int shift, cudaStream_t s) {
+    const int ctas = ctas_per_row(a.rows, a.vocab, sizeof(T));
+    if (!ctas) return false;
     const size_t smem = std::max<size_t>((size_t)(((a.vocab + kVec<T> - 1) / kVec<T> + ctas - 1) / ctas) * 16, 2 * kList * 8);
     static bool ready[64] = {};
     int device = 0;
@@ -873,6 +880,8 @@ bool launch_cluster(const SampleArgs& a, int shift, cudaStream_t s) {
 }
 
 }  // namespace
+
+int sample_plan(int64_t rows, int64_t vocab, int dtype) { return ctas_per_row(rows, vocab, dtype == ENGINE_F32 ? 4 : 2); }
 
 void launch_sample(const SampleArgs& a, cudaStream_t s) {
     if (a.rows == 0) return;
