@@ -258,6 +258,14 @@ ENGINE_API EngineStatus engine_matmul_grouped_fp8_device(const void* d_a, int64_
                                                          const int32_t* d_offsets, int64_t experts, void* d_out,
                                                          int64_t ldo, int32_t out_dtype, int64_t rows, int64_t n,
                                                          int64_t k, int32_t device, void* stream);
+/* For tests and measurements, without a GPU: the form of kernel that the calls above take
+ * (experts 0: one weight) on a GPU of `sms` SMs that holds clusters[0..2] clusters of 2, 4
+ * and 8 CTAs at once; aligned_out: output rows start at multiples of 16 bytes. plan[0]:
+ * CTAs of a wide tile, 1 or 2, or 0 for a narrow one; plan[1]: its tokens; plan[2]: CTAs
+ * that share the k-blocks of a narrow tile. */
+ENGINE_API EngineStatus engine_matmul_fp8_plan(int64_t m, int64_t n, int64_t k, int64_t experts, int32_t out_dtype,
+                                               int32_t aligned_out, int32_t sms, const int32_t clusters[3],
+                                               int32_t plan[3]);
 
 /* One token per row of d_logits [rows, vocab] (F32, F16 or BF16; NaN counts as -inf).
  * w = exp((logit - largest) / temperature), Z = sum of w. In the order of falling

@@ -99,6 +99,7 @@ _SIGS = {
     "engine_matmul_grouped_fp8_device": ([vp, i64, vp, i64, vp, i64, i64, vp, i64, i64, vp, i64, vp, i64, i32, i64,
                                           i64, i64, i32, vp], C.c_int),
     "engine_sample_device": ([vp, i64, i32, vp, i64, vp, vp, vp, vp, i64, i64, vp, vp, i32, vp], C.c_int),
+    "engine_matmul_fp8_plan": ([i64, i64, i64, i64, i32, i32, i32, P(i32), P(i32)], C.c_int),
     "engine_sample_plan": ([i64, i64, i32, P(i32)], C.c_int),
     "engine_ops_relu": ([vp], C.c_int), "engine_ops_silu": ([vp], C.c_int),
     "engine_ops_sigmoid": ([vp], C.c_int), "engine_ops_tanh": ([vp], C.c_int),

@@ -167,6 +167,30 @@ ENGINE_API EngineStatus engine_matmul_grouped_fp8_device(const void* d_a, int64_
     });
 }
 
+ENGINE_API EngineStatus engine_matmul_fp8_plan(int64_t m, int64_t n, int64_t k, int64_t experts, int32_t out_dtype,
+                                               int32_t aligned_out, int32_t sms, const int32_t clusters[3],
+                                               int32_t plan[3]) {
+    return guarded([&]() -> EngineStatus {
+        clear_error();
+        need_extent(m, "matmul_fp8: bad number of rows");
+        need_extent(n, "matmul_fp8: bad number of columns");
+        need_extent(k, "matmul_fp8: bad inner extent");
+        need(m > 0 && n > 0 && k > 0 && experts >= 0 && experts <= 1024, ENGINE_ERR_INVALID_SHAPE, "matmul_fp8: nothing to plan");
+        need(float_type(out_dtype), ENGINE_ERR_INVALID_ARG, "matmul_fp8: the output type must be F32, F16 or BF16");
+        need(sms >= 2, ENGINE_ERR_INVALID_ARG, "matmul_fp8: too few SMs");
+        need(clusters && plan, ENGINE_ERR_NULL_PTR, "matmul_fp8: nowhere to put the plan");
+        static const int32_t none = 0;
+        MatmulFp8Args p;
+        p.m = m; p.n = n; p.k = k; p.out_dtype = out_dtype;
+        if (experts) { p.offsets = &none; p.experts = experts; }       // not read
+        const int32_t held[3] = {clusters[0], clusters[1], clusters[2]};
+        int32_t found[3];
+        matmul_fp8_plan(p, aligned_out != 0, sms, held, found);
+        for (int i = 0; i < 3; ++i) plan[i] = found[i];
+        return ENGINE_OK;
+    });
+}
+
 ENGINE_API EngineStatus engine_sample_device(const void* d_logits, int64_t logits_stride, int32_t dtype,
                                              const float* d_noise, int64_t noise_stride, const float* d_temperature,
                                              const int32_t* d_top_k, const float* d_top_p, const float* d_min_p,

@@ -237,6 +237,9 @@ struct MatmulFp8Args {
     int out_dtype = 0;
 };
 void launch_matmul_fp8(const MatmulFp8Args& p, cudaStream_t s);
+// What launch_matmul_fp8 takes on a GPU of `sms` SMs that holds clusters[0..2] clusters of 2, 4 and 8
+// CTAs: CTAs of a wide tile (0: narrow), tokens of a tile, CTAs over which its k-blocks are split.
+void matmul_fp8_plan(const MatmulFp8Args& p, bool aligned_out, int sms, const int32_t (&clusters)[3], int32_t (&plan)[3]);
 
 // One token per row of logits [rows, vocab]; see engine_sample_device.
 struct SampleArgs {

@@ -1038,12 +1038,18 @@ struct Plan { int wide, bt, split; };
 // the busiest CTA is waves * (k-blocks * time of one + time to store the tile), or with a split
 // the k-blocks' and the joining's, and the least wins. The times (us) are fits to a sweep on
 // a B200, which they meet within 10% or so; the plan's time is within 9% of the best one's for 469
-// shapes of a sweep (mean 0.5%). Measured, m x n x k, bf16 out: 16 x 4096 x 4096: 16 tokens over 4 CTAs
+// shapes of a sweep up to 8192 x 8192 x 8192 (mean 0.5%). Measured, m x n x k, bf16 out: 16 x 4096 x 4096: 16 tokens over 4 CTAs
 // 7.5, over 2 9.1, over 1 12.3; 333 x 2048 x 272: 64: 5.3, 32: 5.8, 128: 6.3, wide 6.9; 2000 x 4096 x 1024:
 // wide 15.3, 128: 20.9, 64: 23.3. Rows that do not start at multiples of 16 bytes: 2000 x 4097 x 1024: wide
 // 19.2, 128: 22.0; f32 4000 x 4097 x 1024: 128: 43.6, 64: 46.4, wide 51.4. Pairs where wide tiles are
-// more than one wave: 8192 x 8192 x 4096 267 against 277.
-Plan plan_matmul(const MatmulFp8Args& g, int64_t experts, int sms, int device, bool wide_out) {
+// more than one wave: 8192 x 8192 x 4096 267 against 277; 129 x 128256 x 4096 139 against 151. But where an
+// odd number of 128-token tiles leaves half of the last pairs empty, single CTAs make fewer waves: 100 x
+// 128256 x 4096 103, pairs 138, 128: 107; 300 x 50264 x 4096 86, pairs 115; 640 x 28672 x 8192 159, pairs 180. Over 75
+// shapes of 48 to 1000 tokens with 28672 to 151936 weight rows the plan is within 7% of the best (mean 1%), but for
+// 100 x 50264 x 4096 with f32 out (56, 128: 50).
+// at_once(split): the clusters of `split` CTAs that run at once.
+template <typename F>
+Plan plan_matmul(const MatmulFp8Args& g, int64_t experts, int sms, bool wide_out, F at_once) {
     if (g.offsets) {
         // The experts' shares are on the GPU; what is known is the average. Measured, as the mean over
         // 15 shapes of the time over the best tile's (8 to 64 experts, even and uneven, 1024 to 2048 wide,
@@ -1059,16 +1065,18 @@ Plan plan_matmul(const MatmulFp8Args& g, int64_t experts, int sms, int device, b
         return Plan{0, r <= 80 ? 64 : 128, 1};
     }
     const int64_t nkb = (g.k + kBlock - 1) / kBlock, n_tiles = (g.n + kTileN - 1) / kTileN;
-    auto waves = [&](int64_t tiles) { return (tiles + sms - 1) / sms; };
-    const int64_t wide_tiles = (g.m + 127) / 128 * ((g.n + kWideN - 1) / kWideN);
-    Plan best{wide_tiles > sms ? 2 : 1, 128, 1};
-    double least = (double)waves(wide_tiles) * (nkb * 0.505 + (wide_out ? 2.2 : g.out_dtype == ENGINE_F32 ? 8.7 : 4.5));
+    auto waves = [&](int64_t tiles, int ctas = 1) { return (tiles + sms / ctas - 1) / (sms / ctas); };
+    auto wide_tiles = [&](int ctas) { return (g.m + 128 * ctas - 1) / (128 * ctas) * ((g.n + kWideN - 1) / kWideN); };
+    // a pair's tile takes as long as a single CTA's, but it has the tokens of two
+    const int wide = wide_tiles(1) > sms && waves(wide_tiles(2), 2) <= waves(wide_tiles(1)) ? 2 : 1;
+    Plan best{wide, 128, 1};
+    double least = (double)waves(wide_tiles(wide), wide) * (nkb * 0.505 + (wide_out ? 2.2 : g.out_dtype == ENGINE_F32 ? 8.7 : 4.5));
     static const struct { int bt; double block, store, join; } kTiles[] = {
         {128, 0.345, 2.3, 5.7}, {64, 0.264, 1.05, 3.1}, {32, 0.24, 0.65, 2.2}, {16, 0.237, 0.55, 1.7}};
     for (const auto& c : kTiles) {
         const int64_t tiles = (g.m + c.bt - 1) / c.bt * n_tiles;
         for (int split = 1; split <= 8; split *= 2) {
-            if (split > 1 && (nkb < 2 * split || tiles * split > sms || tiles > clusters_at_once(split, device))) break;
+            if (split > 1 && (nkb < 2 * split || tiles * split > sms || tiles > at_once(split))) break;
             const double t = split == 1 ? (double)waves(tiles) * (nkb * c.block + c.store) : (double)((nkb + split - 1) / split) * c.block + c.join;
             if (t < least) { least = t; best = Plan{0, c.bt, split}; }
         }
@@ -1077,6 +1085,11 @@ Plan plan_matmul(const MatmulFp8Args& g, int64_t experts, int sms, int device, b
 }
 
 }  // namespace
+
+void matmul_fp8_plan(const MatmulFp8Args& g, bool aligned_out, int sms, const int32_t (&clusters)[3], int32_t (&plan)[3]) {
+    const Plan p = plan_matmul(g, g.offsets ? g.experts : 1, sms, aligned_out, [&](int split) { return clusters[split == 2 ? 0 : split == 4 ? 1 : 2]; });
+    plan[0] = p.wide; plan[1] = p.wide ? 128 * p.wide : p.bt; plan[2] = p.split;
+}
 
 void launch_matmul_fp8(const MatmulFp8Args& g, cudaStream_t s) {
     if (g.m == 0 || g.n == 0) return;
@@ -1136,7 +1149,7 @@ void launch_matmul_fp8(const MatmulFp8Args& g, cudaStream_t s) {
     p.wait_limit = 1000000000LL;
 
     p.wide_out = reinterpret_cast<uintptr_t>(g.out) % 16 == 0 && (g.m <= 1 || g.ldo * (g.out_dtype == ENGINE_F32 ? 4 : 2) % 16 == 0);
-    const Plan plan = plan_matmul(g, experts, sms, device, p.wide_out);
+    const Plan plan = plan_matmul(g, experts, sms, p.wide_out, [&](int split) { return clusters_at_once(split, device); });
     const int wide = plan.wide, bt = wide ? 128 : plan.bt;
     const int tokens = wide ? 128 * wide : bt;
     p.m_tiles = (int)((g.m + tokens - 1) / tokens);

@@ -37,3 +37,43 @@ def test_sample_rows_that_no_cluster_holds():
     assert N.lib().engine_sample_plan(4, 0, F32, C.byref(C.c_int32())) == 6
     assert N.lib().engine_sample_plan(4, 10, 5, C.byref(C.c_int32())) == 7
     assert N.lib().engine_sample_plan(4, 10, F32, None) == 1
+
+
+def matmul_plan(m, n, k, experts=0, dtype=BF16, aligned=True, sms=148, clusters=(74, 35, 16)):
+    """(CTAs of a wide tile or 0, tokens of a tile, CTAs of a split)"""
+    held, plan = (C.c_int32 * 3)(*clusters), (C.c_int32 * 3)()
+    assert N.lib().engine_matmul_fp8_plan(m, n, k, experts, dtype, aligned, sms, held, plan) == 0
+    return tuple(plan)
+
+
+def wide_waves(m, n, pair):
+    tiles = -(-m // (128 * pair)) * -(-n // 256)
+    return -(-tiles // (148 // pair))
+
+
+@pytest.mark.parametrize("n,k", [(4096, 4096), (8192, 4096), (28672, 8192), (50264, 4096), (128256, 4096), (151936, 2048)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_pairs_never_make_more_waves_than_single_ctas(n, k, dtype):
+    """A pair's tile is 256 tokens: with few of them, or an odd number of 128s, its second half is empty."""
+    seen = set()
+    for m in [*range(1, 700, 9), 128, 129, 256, 257, 384, 640, 1000, 4096, 8192]:
+        wide, tokens, split = matmul_plan(m, n, k, dtype=dtype)
+        seen.add(wide)
+        if wide == 2:
+            assert m > 128 and tokens == 256 and wide_waves(m, n, 2) <= wide_waves(m, n, 1), m
+    assert 2 in seen
+
+
+def test_plan_of_head_shapes():
+    assert matmul_plan(100, 128256, 4096) == (1, 128, 1)
+    assert matmul_plan(300, 50264, 4096) == (1, 128, 1)
+    assert matmul_plan(256, 128256, 4096) == (2, 256, 1)
+    assert matmul_plan(8192, 8192, 4096) == (2, 256, 1)
+
+
+def test_plan_refusals():
+    held, plan = (C.c_int32 * 3)(74, 35, 16), (C.c_int32 * 3)()
+    call = N.lib().engine_matmul_fp8_plan
+    assert call(0, 1, 1, 0, F32, 1, 148, held, plan) == 6 and call(1, 1, 1, 1025, F32, 1, 148, held, plan) == 6
+    assert call(1, 1, 1, 0, 3, 1, 148, held, plan) == 7 and call(1, 1, 1, 0, F32, 1, 1, held, plan) == 7
+    assert call(1, 1, 1, 0, F32, 1, 148, None, plan) == 1 and call(1, 1, 1, 0, F32, 1, 148, held, None) == 1
