@@ -54,6 +54,7 @@ struct TcArgs {
     void* out; int64_t ldo; int out_dtype;
     uint32_t table_bytes;               // the experts' tile table in shared memory (12 KB for the most experts)
     int wide_out;                       // output rows start at multiples of 16 bytes
+    int tma_end;                        // TMA may store columns that end here at most
     int* err;
     long long wait_limit;
 };
@@ -589,8 +590,8 @@ static_assert(128 * kWideRegsLess + 32 * kWideEpi * kWideRegsMore <= kWideThread
 // The warp's 32 rows (one per lane) of kWideCols sums to rows of the output, `rows` of which
 // are this tile's: through the warp's own shared memory in chunks of 128 bytes per row, whose
 // 16-byte pieces are swizzled against bank conflicts in the pattern of the output's tensor map.
-// Full tiles leave by TMA while the warp goes on; rows that are not aligned for it, or
-// belong to the next expert, are copied out by the warp. One fence and one pair of TMA
+// Full tiles leave by TMA while the warp goes on; rows that are not aligned for it, or belong to
+// the next expert, and last columns that end inside 16 bytes are copied out by the warp. One fence and one pair of TMA
 // stores per 256 bytes of a row: issuing them takes a warp some 400 cycles (a tile of 8192 x
 // 8192 x 4096 has 32000).
 constexpr int kWideChunk = 32 * 128, kWideChunks = 2, kWideStage = kWideChunks * kWideChunk;
@@ -617,9 +618,9 @@ __device__ __forceinline__ void wide_store(const TcArgs& p, const CUtensorMap* t
                                            int row0, int rows, int n0) {
     constexpr int kPer = 128 / sizeof(T), kPiece = 16 / sizeof(T);   // values of a chunk's row and of a piece
     const int lane = threadIdx.x & 31;
-    const bool tma = p.wide_out && rows >= 32;
 #pragma unroll
     for (int c = 0; c < kWideCols; c += kWideChunks * kPer) {
+        const bool tma = rows >= 32 && n0 + c + kWideChunks * kPer <= p.tma_end;
         if (lane == 0) bulk_wait_read<0>();                          // what was here has left
         __syncwarp();
 #pragma unroll
@@ -1149,6 +1150,8 @@ void launch_matmul_fp8(const MatmulFp8Args& g, cudaStream_t s) {
     p.wait_limit = 1000000000LL;
 
     p.wide_out = reinterpret_cast<uintptr_t>(g.out) % 16 == 0 && (g.m <= 1 || g.ldo * (g.out_dtype == ENGINE_F32 ? 4 : 2) % 16 == 0);
+    // TMA cuts the end of a row to whole 16 bytes: it would reach beyond rows that end inside them
+    p.tma_end = !p.wide_out ? 0 : g.n * (g.out_dtype == ENGINE_F32 ? 4 : 2) % 16 ? p.n : 0x7FFFFFFF;
     const Plan plan = plan_matmul(g, experts, sms, p.wide_out, [&](int split) { return clusters_at_once(split, device); });
     const int wide = plan.wide, bt = wide ? 128 : plan.bt;
     const int tokens = wide ? 128 * wide : bt;
