@@ -77,3 +77,41 @@ def test_plan_refusals():
     assert call(0, 1, 1, 0, F32, 1, 148, held, plan) == 6 and call(1, 1, 1, 1025, F32, 1, 148, held, plan) == 6
     assert call(1, 1, 1, 0, 3, 1, 148, held, plan) == 7 and call(1, 1, 1, 0, F32, 1, 1, held, plan) == 7
     assert call(1, 1, 1, 0, F32, 1, 148, None, plan) == 1 and call(1, 1, 1, 0, F32, 1, 148, held, None) == 1
+
+
+# m, n, k and the plan for 32- and for 16-bit outputs: every form of the product's kernels, with
+# several tiles per CTA, partial tiles and blocks, and output rows aligned or not. The GPU tests
+# compute these, so a refit that changes a plan shows here.
+FORMS = [
+    (2600, 5000, 400, (2, 256, 1), (2, 256, 1)), (520, 9000, 640, (2, 256, 1), (2, 256, 1)),
+    (20000, 304, 130, (2, 256, 1), (2, 256, 1)), (2000, 2600, 300, (2, 256, 1), (2, 256, 1)),
+    (1500, 5001, 4000, (2, 256, 1), (2, 256, 1)), (2600, 5001, 400, (0, 128, 1), (2, 256, 1)),
+    (300, 20000, 400, (1, 128, 1), (1, 128, 1)), (700, 4000, 256, (1, 128, 1), (1, 128, 1)),
+    (777, 3001, 4000, (1, 128, 1), (1, 128, 1)),
+    (5, 40000, 256, (0, 16, 1), (0, 16, 1)), (20, 45000, 130, (0, 32, 1), (0, 32, 1)),
+    (33, 40000, 400, (0, 64, 1), (0, 64, 1)), (300, 6000, 1000, (0, 128, 1), (0, 128, 1)),
+    (16, 5000, 2064, (0, 16, 2), (0, 16, 2)), (129, 203, 1040, (0, 16, 4), (0, 16, 4)), (50, 128, 4096, (0, 16, 8), (0, 16, 8)),
+    (255, 640, 2064, (0, 32, 2), (0, 32, 2)), (257, 383, 2064, (0, 32, 4), (0, 32, 4)), (161, 200, 3000, (0, 32, 8), (0, 32, 8)),
+    (255, 1279, 4096, (0, 64, 2), (0, 64, 2)), (257, 640, 4096, (0, 64, 4), (0, 64, 4)), (300, 203, 8192, (0, 64, 8), (0, 64, 8)),
+    (255, 2600, 8192, (0, 128, 2), (0, 128, 2)), (255, 1279, 8192, (0, 128, 4), (0, 128, 4)),
+]
+# rows, experts, n, k: grouped plans
+GROUP_FORMS = [
+    (500, 64, 1300, 272, (0, 16, 1), (0, 16, 1)), (500, 33, 1300, 272, (0, 32, 1), (0, 32, 1)), (1500, 1024, 130, 128, (0, 16, 1), (0, 16, 1)),
+    (2500, 200, 700, 400, (0, 32, 1), (0, 32, 1)), (2000, 64, 1301, 272, (0, 64, 1), (0, 64, 1)), (9000, 200, 300, 256, (0, 64, 1), (0, 64, 1)),
+    (9000, 33, 1104, 400, (1, 128, 1), (1, 128, 1)), (9001, 65, 1101, 400, (0, 128, 1), (1, 128, 1)), (6500, 70, 900, 1040, (1, 128, 1), (0, 128, 1)),
+]
+
+
+@pytest.mark.parametrize("clusters", [(74, 35, 16), (60, 28, 12), (74, 37, 18)])
+def test_plans_of_the_computed_forms(clusters):
+    for m, n, k, f32, f16 in FORMS:
+        for dtype, want in ((F32, f32), (F16, f16), (BF16, f16)):
+            aligned = n * (4 if dtype == F32 else 2) % 16 == 0
+            assert matmul_plan(m, n, k, dtype=dtype, aligned=aligned, clusters=clusters) == want, (m, n, k, dtype)
+    for rows, experts, n, k, f32, f16 in GROUP_FORMS:
+        for dtype, want in ((F32, f32), (F16, f16), (BF16, f16)):
+            aligned = n * (4 if dtype == F32 else 2) % 16 == 0
+            assert matmul_plan(rows, n, k, experts, dtype, aligned, clusters=clusters) == want, (rows, experts, n, k, dtype)
+    plans = {p for form in FORMS for p in form[3:]}
+    assert plans == {(2, 256, 1), (1, 128, 1), *((0, t, s) for t in (16, 32, 64, 128) for s in (1, 2, 4, 8))} - {(0, 128, 8)}
