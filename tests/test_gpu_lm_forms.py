@@ -140,3 +140,30 @@ def test_two_threads():
     for t in threads:
         t.join()
     assert len(done) == 2 and not wrong
+
+
+def test_offsets_beyond_32_bits():
+    """The last rows of arrays of more than 2^31 elements."""
+    g = gen(5)
+    rows, cols = 270000, 8191
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda")
+    x[:2], x[-3:] = randn(g, 2, cols).bfloat16(), randn(g, 3, cols).bfloat16()
+    w = torch.ones(cols, dtype=torch.bfloat16, device="cuda")
+    y64, _ = base.norm_ref(x[-3:], w, None, 1e-5)
+    y = pb.ops_rms_norm(x, w, eps=1e-5)[-3:]
+    assert ((y.double() - y64).abs() <= (96 * base.U + 2.0 ** -8) * y64.abs() * 1.0001).all()
+    del x
+    m, n, k = 17000, 131072, 128
+    a, sa, b, sb = operands(g, m, n, k)
+    out = pb.ops_matmul_fp8(a, sa, b, sb)
+    for lo in (0, 16250, 16990):
+        check_product(out[lo:lo + 10], a[lo:lo + 10], sa[lo:lo + 10], b, sb)
+    tail = out[-40:].float()
+    e = torch.empty(m, n, device="cuda")
+    e[-40:].exponential_(generator=g)
+    t = torch.full((m,), 0.9, device="cuda")
+    t[:-40] = 0
+    tok, prob = pb.ops_sample(out, e, temperature=t)
+    want = pb.ops_sample(out[-40:].clone(), e[-40:].clone(), temperature=t[-40:].clone())
+    assert torch.equal(tok[-40:], want[0]) and torch.allclose(prob[-40:], want[1], rtol=1e-4, atol=1e-37)
+    assert torch.equal(tok[:40].long(), out[:40].float().argmax(1)) and tail.isfinite().all()
