@@ -49,23 +49,23 @@ constexpr int kGroup = 128;
 // bits hold, so they must not be off by an ulp. (Bit by bit the division's bytes and scales. On
 // pairs the step costs next to nothing: 16384 x 8192 bf16, residual: 139.7 us, 139.1 without it,
 // 176 with divisions; 5000 x 4096 f32 27.3, 26.5 and 31.4.) The residue of an infinite scale would be
-// NaN, so `finite` stands for it there. A quarter of both in the inverse, since the fast division
+// NaN, so a finite one stands for it there. A quarter of both in the inverse, since the fast division
 // takes divisors to 2^126.
 struct Scale {
-    float s, inv, finite;
+    float s, inv, minus;
 };
 __device__ __forceinline__ Scale scale_of(float m) {
-    constexpr float c = 1.0f / kE4m3Max;
+    constexpr float c = 1.0f / kE4m3Max, most = 3.0e38f;
     Scale d;
-    const float s = m * c;
-    d.s = s == INFINITY ? s : fmaf(fmaf(-kE4m3Max, s, m), c, s);
+    const float s = fminf(m * c, most);
+    d.s = fmaf(fmaf(-kE4m3Max, s, m), c, s);
     d.inv = __fdividef(0.25f * kE4m3Max, 0.25f * m);
-    d.finite = fminf(d.s, 3.0e38f);
+    d.minus = fmaxf(-d.s, -most);
     return d;
 }
-__device__ __forceinline__ float2 quotients(float2 v, float2 inv, float2 finite) {
+__device__ __forceinline__ float2 quotients(float2 v, float2 inv, float2 minus) {
     const float2 q = __fmul2_rn(v, inv);
-    return __ffma2_rn(__ffma2_rn(make_float2(-q.x, -q.y), finite, v), inv, q);
+    return __ffma2_rn(__ffma2_rn(q, minus, v), inv, q);
 }
 __device__ __forceinline__ float2 times(float2 h, float r, float2 w) { return __fmul2_rn(__fmul2_rn(h, make_float2(r, r)), w); }
 __device__ __forceinline__ uint32_t four_fp8(float2 a, float2 b) {
@@ -426,11 +426,11 @@ rms_norm_kernel(RmsNormArgs a) {
             const Scale d = scale_of(m);
             if (c < cols && c % kGroup == 0) a.scales[row * a.scales_stride + c / kGroup] = d.s;
             uint32_t b[2] = {0, 0};
-            const float2 inv = make_float2(d.inv, d.inv), finite = make_float2(d.finite, d.finite);
+            const float2 inv = make_float2(d.inv, d.inv), minus = make_float2(d.minus, d.minus);
 #pragma unroll
             for (int j = 0; j < P; j += 4)
-                b[j / 4] = four_fp8(quotients(make_float2(v[i][j], v[i][j + 1]), inv, finite),
-                                    quotients(make_float2(v[i][j + 2], v[i][j + 3]), inv, finite));
+                b[j / 4] = four_fp8(quotients(make_float2(v[i][j], v[i][j + 1]), inv, minus),
+                                    quotients(make_float2(v[i][j + 2], v[i][j + 3]), inv, minus));
             out[i] = make_uint4(b[0], b[1], 0, 0);
             if (ALIGNED && c < cols) {
                 uint8_t* y = static_cast<uint8_t*>(a.y) + row * a.y_stride + c;
@@ -615,7 +615,7 @@ rms_norm_alike_kernel(RmsNormArgs a) {
                 for (int t = 0; t < 4; t += 2) {
                     const Scale &d0 = j + t < S.value ? d_end : d_own, &d1 = j + t + 1 < S.value ? d_end : d_own;
                     f[t / 2] = quotients(make_float2(v[i][j + t], v[i][j + t + 1]), make_float2(d0.inv, d1.inv),
-                                         make_float2(d0.finite, d1.finite));
+                                         make_float2(d0.minus, d1.minus));
                 }
                 b[j / 4] = four_fp8(f[0], f[1]);
             }
