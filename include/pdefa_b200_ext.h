@@ -227,8 +227,9 @@ ENGINE_API EngineStatus pdefa_batch_wait(PdefaBatchRunner* runner, int64_t ticke
  * or F32. d_h (may be NULL, may be d_x or d_residual itself) receives h rounded to
  * dtype; y is computed from the unrounded h. With d_scales the output is 8-bit: d_y
  * holds e4m3 bytes, d_scales one float for each 128 columns of a row,
- * scale = max(largest |y| of the 128, 1e-10) / 448, byte = e4m3(y / scale). A row with
- * a NaN or an infinity gives NaN. */
+ * scale = max(largest |y| of the 128, 1e-10) / 448, byte = e4m3(y / scale), both as a
+ * 32-bit division rounds them. A row with a NaN gives NaN. An infinite h makes the root
+ * infinite: its own y is NaN (and with it the 8-bit group and its scale), the others 0. */
 ENGINE_API EngineStatus engine_rms_norm_device(const void* d_x, int64_t x_stride, const void* d_residual,
                                                int64_t residual_stride, const void* d_weight, void* d_h,
                                                int64_t h_stride, void* d_y, int64_t y_stride, float* d_scales,
@@ -270,8 +271,9 @@ ENGINE_API EngineStatus engine_matmul_fp8_plan(int64_t m, int64_t n, int64_t k, 
 /* One token per row of d_logits [rows, vocab] (F32, F16 or BF16; NaN counts as -inf).
  * w = exp((logit - largest) / temperature), Z = sum of w. In the order of falling
  * logits (equal ones by rising index) a token is kept if fewer than top_k tokens come
- * before it, the mass before it is below top_p * Z, w >= min_p and w > 0; the first
- * token is always kept. Of the kept tokens the one with the largest w / noise wins
+ * before it, the mass before it is below top_p * Z (of the whole row's mass, also with
+ * top_k), w >= min_p and w > 0 (a w under 2^-126 may count as 0); the first token is
+ * always kept. Of the kept tokens the one with the largest w / noise wins
  * (lowest index among equals): with noise [rows, vocab] of independent exponential
  * variates, token i is drawn with probability w_i / (sum of kept w). Negative (-0
  * too) or NaN noise takes its token out of the race.

@@ -23,8 +23,9 @@
 // What bounds them (B200). Few tokens: reading the weights, 64 rows over 64 experts of 2048 x
 // 2048 in 31 us, 5.4 TB/s; for one weight of 16 MB a launch and the pipeline's ends are most of
 // 6.2 us. Many tokens: TMEM, which the epilogue reads (128 KB per k-block and SM) beside the
-// tensor core; 8192 x 8192 x 4096 takes 267 us, 2060 TFLOP/s, at 990 cycles per k-block, where
-// products alone, without loads and epilogue, need 640 and the epilogue's reads 350.
+// tensor core; 8192 x 8192 x 4096 takes 268 us from a graph, 2050 TFLOP/s (278 on a slower card;
+// 310 in a loop of calls, where the power limit rules), at 990 cycles per k-block, where products
+// alone, without loads and epilogue, need 640 and the epilogue's reads 350.
 #include <algorithm>
 #include <atomic>
 #include <cuda.h>

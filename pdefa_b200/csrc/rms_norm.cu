@@ -6,10 +6,11 @@
 //   8-bit: scale = max(max|y| over 128 columns, 1e-10) / 448, q = e4m3(y / scale)
 //
 // Bound by memory: the values are read once and written once, 16384 x 8192 bf16 with a
-// residual and an 8-bit output in 139 us (6.8 TB/s, 105% of a plain copy's rate on B200).
+// residual and an 8-bit output in 140 us from a graph (6.8 TB/s, 105% of a plain copy's rate on
+// B200) and 157 in a loop of calls (6.0 TB/s).
 //
-// The statistic and the scales come from the unrounded 32-bit sum. A NaN in a row
-// makes its whole output NaN (an infinity makes the statistic 0 and itself NaN).
+// The statistic and the scales come from the unrounded 32-bit sum. A NaN in a row makes its
+// whole output NaN. An infinity makes the root infinite: it becomes NaN, the row's others 0.
 #include <algorithm>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -480,7 +481,7 @@ __device__ __forceinline__ void by_offset(int s, F f) {
 // on beyond the row, and written by halves. The order in which the squares are added depends on s.
 // Bound by its instructions and its barriers, so registers are limited, to 40 with two or three pieces
 // a thread, for two CTAs of 544 threads on an SM or four of 352 (4000 x 8191 bf16, residual, 8-bit output:
-// 54 us, over two pieces 59, with one CTA on an SM 96, the general kernel 84; 4000 x 8190, 16-bit
+// 53 us, over two pieces 59, with one CTA on an SM 96, the general kernel 84; 4000 x 8190, 16-bit
 // output: 43, general 84; 16000 x 2049, 8-bit: 50 against 57; 509 x 2050 f16: 2.6 against 3.0). Weights read
 // early pay with one piece a thread only (2.6 against 2.75; 55 against 51 with two).
 template <typename T, typename W, int N, bool QUANT>

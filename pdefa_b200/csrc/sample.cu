@@ -22,7 +22,7 @@
 //
 // A row is read once into the shared memory of a cluster. What bounds it is not that read but
 // the phases after it, each a barrier and an exchange over the cluster's CTAs (1 to 1.3 us):
-// 256 x 131072 bf16 with top-k, top-p and min-p 50 us (1.3 TB/s; the read alone 10), one row of
+// 256 x 131072 bf16 with top-k, top-p and min-p 51 us (1.3 TB/s; the read alone 10), one row of
 // 32000 6.4 us. So rows are spread over CTAs to have all of them in flight at once, candidates are
 // counted before they are listed, and what one CTA can finish alone is sent to one.
 #include <algorithm>
